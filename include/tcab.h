@@ -108,7 +108,12 @@ typedef struct tcab_chain {
 /* Epilogue of the contraction (the piped map after the K reduction). */
 typedef enum tcab_act {
   TCAB_ACT_NONE = 0,
-  TCAB_ACT_RELU = 1 /* fmaxf(v, 0) */
+  TCAB_ACT_RELU = 1, /* fmaxf(v, 0) */
+  /* tcab_gemm_bias_act_residual, tcab_gated_gemm and their backward passes only: */
+  TCAB_ACT_SILU = 2,      /* v / (1 + exp(-v))                                               */
+  TCAB_ACT_GELU = 3,      /* v Phi(v), Phi the normal distribution (erf)                     */
+  TCAB_ACT_GELU_TANH = 4, /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2               */
+  TCAB_ACT_SIGMOID = 5    /* 1 / (1 + exp(-v)); the gated forms only                         */
 } tcab_act;
 
 /* Message of the calling thread's last failed call ("" if none). Replaces the text of the
@@ -273,6 +278,69 @@ TCAB_API int tcab_layernorm_rows(const tcab_tensor* x, const tcab_tensor* gamma,
  * Requires K % 8 == 0, N % 8 == 0 and 16-byte aligned base pointers (TMA tensor maps). */
 TCAB_API int tcab_gemm_bias_act(const tcab_tensor* a, const tcab_tensor* b, const tcab_tensor* bias,
                        int act, const tcab_tensor* c, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------
+ * A feed-forward sublayer and its training step. The reference has no backward passes and no such layer; these stand
+ * beside tcab_layernorm_rows and tcab_gemm_bias_act and follow their rules. None of them allocates: a backward pass takes
+ * a workspace of at least the bytes its _workspace function gives (16-byte aligned device memory on the current device,
+ * free to be reused once the call's work on the stream is done; two calls that may overlap on the GPU need one each).
+ * An output must not overlap another output or an input; where a comment names an input that an output may be, the two
+ * must start at the same address. Every sum is fp32 and taken in a fixed order: the same call gives the same bits.
+ * --------------------------------------------------------------------------------------------------- */
+
+/* tcab_layernorm_rows that also stores each row's statistics: mean and rstd = 1 / sqrtf(var + eps), fp32, with the
+ * extents of x without the innermost one (rank-1 x: extent 1). y has the bits tcab_layernorm_rows gives; y may be x.
+ * The innermost extent must be positive. */
+TCAB_API int tcab_layernorm_rows_stats(const tcab_tensor* x, const tcab_tensor* gamma, const tcab_tensor* beta, float eps,
+                                       const tcab_tensor* y, const tcab_tensor* mean, const tcab_tensor* rstd, void* stream);
+
+/* Its backward pass. With u = (x - mean) * rstd and w = dy * gamma:
+ *   dx = rstd * (w - sum(w) / n - u * sum(w * u) / n),  dgamma = sum over rows of dy * u,  dbeta = sum over rows of dy.
+ * dy, x, dx: bf16 or fp32, one type and shape; gamma: rank 1, the same type; mean, rstd: as stored by the forward pass;
+ * dgamma, dbeta: fp32, rank 1. No rows: dgamma and dbeta are zero. dx may be dy or x. */
+TCAB_API uint64_t tcab_layernorm_rows_backward_workspace(const tcab_tensor* x);
+TCAB_API int tcab_layernorm_rows_backward(const tcab_tensor* dy, const tcab_tensor* x, const tcab_tensor* gamma,
+                                          const tcab_tensor* mean, const tcab_tensor* rstd, const tcab_tensor* dx,
+                                          const tcab_tensor* dgamma, const tcab_tensor* dbeta, void* workspace,
+                                          uint64_t workspace_bytes, void* stream);
+
+/* c = act(a @ b + bias) + residual, and optionally preact = a @ b + bias for the backward pass.
+ * a [M,K], b [K,N], residual [M,N] or NULL, preact [M,N] or NULL, c [M,N]: bf16; bias [N]: fp32 or NULL; fp32
+ * accumulation, every stored value rounded once. act: none, relu, silu, gelu, gelu_tanh. Any M, also 0 and 1; K and N
+ * multiples of 8 and 16-byte aligned tensors, as for tcab_gemm_bias_act. K = 0 gives act(bias) + residual. c may be the
+ * residual. */
+TCAB_API int tcab_gemm_bias_act_residual(const tcab_tensor* a, const tcab_tensor* b, const tcab_tensor* bias,
+                                         const tcab_tensor* residual, int act, const tcab_tensor* preact,
+                                         const tcab_tensor* c, void* stream);
+
+/* Its backward pass: dz = dc * act'(preact), da = dz @ b^T, db = a^T @ dz, dbias = column sums of dz (the gradient of the
+ * residual is dc itself). Each of da [M,K] bf16, db [K,N] bf16, dbias [N] fp32 may be NULL: it is then not computed.
+ * preact may be NULL when act is none. dz is rounded to bf16 as the operand of the two contractions; dbias is summed
+ * from the unrounded values. relu's slope at 0 is 0. */
+TCAB_API uint64_t tcab_gemm_bias_act_backward_workspace(uint32_t m, uint32_t n, int act, int with_dbias);
+TCAB_API int tcab_gemm_bias_act_backward(const tcab_tensor* dc, const tcab_tensor* a, const tcab_tensor* b,
+                                         const tcab_tensor* preact, int act, const tcab_tensor* da, const tcab_tensor* db,
+                                         const tcab_tensor* dbias, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* h = act(x @ w_gate + bias_gate) * (x @ w_up + bias_up): both projections of a gated feed-forward layer, the activation
+ * and the product in one kernel; optionally gate = x @ w_gate + bias_gate and up = x @ w_up + bias_up for the backward
+ * pass (both or neither). x [M,K], w_gate, w_up [K,N], gate, up, h [M,N]: bf16; bias_gate, bias_up [N]: fp32, both or
+ * neither. act: silu, gelu, gelu_tanh, sigmoid, relu. Extents and alignment as for tcab_gemm_bias_act_residual. */
+TCAB_API int tcab_gated_gemm(const tcab_tensor* x, const tcab_tensor* w_gate, const tcab_tensor* w_up,
+                             const tcab_tensor* bias_gate, const tcab_tensor* bias_up, int act, const tcab_tensor* gate,
+                             const tcab_tensor* up, const tcab_tensor* h, void* stream);
+
+/* Its backward pass: dgate = dh * up * act'(gate), dup = dh * act(gate),
+ *   dx = dgate @ w_gate^T + dup @ w_up^T (one accumulator),  dw_gate = x^T @ dgate,  dw_up = x^T @ dup,
+ * and the column sums of dgate and dup. dx [M,K] may be NULL; dw_gate, dw_up [K,N] (bf16) both or neither; dbias_gate,
+ * dbias_up [N] (fp32) both or neither. dgate and dup are rounded to bf16 as operands; the column sums are taken from
+ * the unrounded values. */
+TCAB_API uint64_t tcab_gated_gemm_backward_workspace(uint32_t m, uint32_t n, int with_dbias);
+TCAB_API int tcab_gated_gemm_backward(const tcab_tensor* dh, const tcab_tensor* x, const tcab_tensor* w_gate,
+                                      const tcab_tensor* w_up, const tcab_tensor* gate, const tcab_tensor* up, int act,
+                                      const tcab_tensor* dx, const tcab_tensor* dw_gate, const tcab_tensor* dw_up,
+                                      const tcab_tensor* dbias_gate, const tcab_tensor* dbias_up, void* workspace,
+                                      uint64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------
  * Host buffers: upload, kernel and download pipelined over chunks of the independent axis.

@@ -19,7 +19,7 @@ MAX_BATCH = 32
 
 OK, ERR_INVALID_ARG, ERR_SHAPE, ERR_DTYPE, ERR_ALIGNMENT, ERR_UNSUPPORTED, ERR_CUDA, ERR_TOO_LARGE = range(8)
 F32, BF16, I32, U32 = 0, 1, 2, 3
-ACT_NONE, ACT_RELU = 0, 1
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_SIGMOID = range(6)
 USE_REDUCE, USE_CONTRACT, USE_MAP, USE_REDUCE_BATCHED = 0, 1, 2, 3
 
 
@@ -76,6 +76,18 @@ SYMBOLS = [
      [C.POINTER(Tensor), C.POINTER(Tensor), C.POINTER(Tensor), C.c_float, C.POINTER(Tensor), C.c_void_p]),
     ("tcab_gemm_bias_act", C.c_int,
      [C.POINTER(Tensor), C.POINTER(Tensor), C.POINTER(Tensor), C.c_int, C.POINTER(Tensor), C.c_void_p]),
+    ("tcab_layernorm_rows_stats", C.c_int, [C.POINTER(Tensor)] * 3 + [C.c_float] + [C.POINTER(Tensor)] * 3 + [C.c_void_p]),
+    ("tcab_layernorm_rows_backward_workspace", C.c_uint64, [C.POINTER(Tensor)]),
+    ("tcab_layernorm_rows_backward", C.c_int, [C.POINTER(Tensor)] * 8 + [C.c_void_p, C.c_uint64, C.c_void_p]),
+    ("tcab_gemm_bias_act_residual", C.c_int,
+     [C.POINTER(Tensor)] * 4 + [C.c_int] + [C.POINTER(Tensor)] * 2 + [C.c_void_p]),
+    ("tcab_gemm_bias_act_backward_workspace", C.c_uint64, [C.c_uint32, C.c_uint32, C.c_int, C.c_int]),
+    ("tcab_gemm_bias_act_backward", C.c_int,
+     [C.POINTER(Tensor)] * 4 + [C.c_int] + [C.POINTER(Tensor)] * 3 + [C.c_void_p, C.c_uint64, C.c_void_p]),
+    ("tcab_gated_gemm", C.c_int, [C.POINTER(Tensor)] * 5 + [C.c_int] + [C.POINTER(Tensor)] * 3 + [C.c_void_p]),
+    ("tcab_gated_gemm_backward_workspace", C.c_uint64, [C.c_uint32, C.c_uint32, C.c_int]),
+    ("tcab_gated_gemm_backward", C.c_int,
+     [C.POINTER(Tensor)] * 6 + [C.c_int] + [C.POINTER(Tensor)] * 5 + [C.c_void_p, C.c_uint64, C.c_void_p]),
     ("tcab_device_status", C.c_int, [C.POINTER(C.c_int)]),
     ("tcab_chain_prepare", C.c_int, [C.POINTER(Chain), C.POINTER(C.c_int32), C.c_uint32, C.c_int, C.c_int]),
     ("tcab_map", C.c_int, [C.POINTER(Chain), C.POINTER(Tensor), C.c_uint32, C.POINTER(Tensor), C.c_void_p]),

@@ -16,6 +16,7 @@
 
 #include "../../include/tcab_tuning.h"
 #include "common.cuh"
+#include "ffn_gemm.h"
 #include "rowvec.cuh"
 
 namespace tcab {
@@ -225,6 +226,116 @@ int have_device(const char* op) {
     if (tcab_rc_ != TCAB_OK) return tcab_rc_; \
   } while (0)
 
+uint64_t tensor_bytes(const tcab_tensor* t) { return count(t, 0, t->rank) * (t->dtype == TCAB_BF16 ? 2 : 4); }
+
+// Outputs against everything else a call touches: `outs` first, then the inputs. An output may be exactly the input
+// may_be[i] where that is given. Null entries are skipped.
+struct Named {
+  const char* name;
+  const tcab_tensor* t;
+};
+int need_disjoint(const char* op, const Named* outs, int n_outs, const Named* ins, int n_ins, const tcab_tensor* const* shareable = nullptr,
+                  int n_shareable = 0) {
+  auto overlap = [](const tcab_tensor* a, const tcab_tensor* b) {
+    const uintptr_t pa = reinterpret_cast<uintptr_t>(a->data), pb = reinterpret_cast<uintptr_t>(b->data);
+    const uint64_t na = tensor_bytes(a), nb = tensor_bytes(b);
+    return na > 0 && nb > 0 && pa < pb + nb && pb < pa + na;
+  };
+  for (int i = 0; i < n_outs; ++i) {
+    if (outs[i].t == nullptr) continue;
+    for (int j = i + 1; j < n_outs; ++j)
+      if (outs[j].t != nullptr && overlap(outs[i].t, outs[j].t))
+        return fail(TCAB_ERR_INVALID_ARG, "%s: %s overlaps %s", op, outs[i].name, outs[j].name);
+    for (int j = 0; j < n_ins; ++j) {
+      if (ins[j].t == nullptr || !overlap(outs[i].t, ins[j].t)) continue;
+      bool shared = false;  // the first output alone may be one of `shareable`, from the same address on
+      for (int k = 0; i == 0 && k < n_shareable; ++k) shared = shared || (shareable[k] == ins[j].t && outs[i].t->data == ins[j].t->data);
+      if (!shared) return fail(TCAB_ERR_INVALID_ARG, "%s: %s overlaps %s", op, outs[i].name, ins[j].name);
+    }
+  }
+  return TCAB_OK;
+}
+
+// mean / rstd of x's rows: f32, the extents of x without the innermost one (rank-1 x: extent 1).
+int check_row_stats(const char* op, const char* name, const tcab_tensor* t, const tcab_tensor* x) {
+  TCAB_TRY(check_tensor(op, name, t));
+  TCAB_TRY(need_dtype(op, name, t, TCAB_F32, "f32"));
+  bool ok = x->rank == 1 ? (t->rank == 1 && t->dims[0] == 1) : t->rank == x->rank - 1;
+  for (uint32_t i = 0; ok && x->rank > 1 && i + 1 < x->rank; ++i) ok = t->dims[i] == x->dims[i];
+  if (!ok) return fail(TCAB_ERR_SHAPE, "%s: %s must have the extents of x without the innermost one", op, name);
+  return need_elem_align(op, name, t, 4);
+}
+
+int check_row_param(const char* op, const char* name, const tcab_tensor* t, uint32_t cols, int dtype, const char* spelled) {
+  TCAB_TRY(check_tensor(op, name, t));
+  TCAB_TRY(need_dtype(op, name, t, dtype, spelled));
+  if (t->rank != 1 || t->dims[0] != cols)
+    return fail(TCAB_ERR_SHAPE, "%s: %s must be rank 1 with extent %u (the innermost extent of x)", op, name, cols);
+  return need_elem_align(op, name, t, dtype == TCAB_F32 ? 4 : 2);
+}
+
+// x of the layer-norm forms with statistics.
+int check_norm_rows(const char* op, const tcab_tensor* x) {
+  TCAB_TRY(check_tensor(op, "x", x));
+  if (x->dtype != TCAB_F32 && x->dtype != TCAB_BF16) return fail(TCAB_ERR_DTYPE, "%s: x must be f32 or bf16", op);
+  if (x->dims[x->rank - 1] == 0) return fail(TCAB_ERR_SHAPE, "%s: the innermost extent of x must be positive", op);
+  return need_elem_align(op, "x", x, x->dtype == TCAB_F32 ? 4 : 2);
+}
+
+int check_like_x(const char* op, const char* name, const tcab_tensor* t, const tcab_tensor* x) {
+  TCAB_TRY(check_tensor(op, name, t));
+  if (t->dtype != x->dtype) return fail(TCAB_ERR_DTYPE, "%s: %s must have the element type of x", op, name);
+  if (!same_shape(t, x)) return fail(TCAB_ERR_SHAPE, "%s: %s must have the shape of x", op, name);
+  return need_elem_align(op, name, t, x->dtype == TCAB_F32 ? 4 : 2);
+}
+
+// A bf16 [rows, cols] operand of the feed-forward contractions; optional ones may be null.
+int check_matrix(const char* op, const char* name, const tcab_tensor* t, uint32_t rows, uint32_t cols) {
+  TCAB_TRY(check_tensor(op, name, t));
+  TCAB_TRY(need_dtype(op, name, t, TCAB_BF16, "bf16"));
+  if (t->rank != 2 || t->dims[0] != rows || t->dims[1] != cols)
+    return fail(TCAB_ERR_SHAPE, "%s: %s must be [%u, %u]", op, name, rows, cols);
+  return need_elem_align(op, name, t, 16);
+}
+int check_matrix_opt(const char* op, const char* name, const tcab_tensor* t, uint32_t rows, uint32_t cols) {
+  return t == nullptr ? TCAB_OK : check_matrix(op, name, t, rows, cols);
+}
+int check_bias_opt(const char* op, const char* name, const tcab_tensor* t, uint32_t n) {
+  if (t == nullptr) return TCAB_OK;
+  TCAB_TRY(check_tensor(op, name, t));
+  TCAB_TRY(need_dtype(op, name, t, TCAB_F32, "f32"));
+  if (t->rank != 1 || t->dims[0] != n) return fail(TCAB_ERR_SHAPE, "%s: %s must be [%u]", op, name, n);
+  return need_elem_align(op, name, t, 4);
+}
+// The first two operands of a contraction, a [M,K] and b [K,N]: they name the extents.
+int check_contraction(const char* op, const char* an, const tcab_tensor* a, const char* bn, const tcab_tensor* b, uint32_t* m,
+                      uint32_t* k, uint32_t* n) {
+  TCAB_TRY(check_tensor(op, an, a));
+  TCAB_TRY(check_tensor(op, bn, b));
+  TCAB_TRY(need_dtype(op, an, a, TCAB_BF16, "bf16"));
+  TCAB_TRY(need_dtype(op, bn, b, TCAB_BF16, "bf16"));
+  if (a->rank != 2 || b->rank != 2) return fail(TCAB_ERR_SHAPE, "%s: %s and %s must be rank 2", op, an, bn);
+  if (b->dims[0] != a->dims[1]) return fail(TCAB_ERR_SHAPE, "%s: %s.Dim(0) must equal %s.Dim(1) (dim k)", op, bn, an);
+  *m = a->dims[0];
+  *k = a->dims[1];
+  *n = b->dims[1];
+  if (*k % 8 != 0 || *n % 8 != 0)
+    return fail(TCAB_ERR_ALIGNMENT, "%s: K and N must be multiples of 8 (16-byte rows for the tensor maps)", op);
+  TCAB_TRY(need_elem_align(op, an, a, 16));
+  return need_elem_align(op, bn, b, 16);
+}
+int check_workspace(const char* op, const void* ws, uint64_t have, uint64_t need) {
+  if (have < need || (need > 0 && ws == nullptr))
+    return fail(TCAB_ERR_INVALID_ARG, "%s: the workspace has %llu bytes, %llu are needed", op,
+                static_cast<unsigned long long>(ws != nullptr ? have : 0), static_cast<unsigned long long>(need));
+  if (reinterpret_cast<uintptr_t>(ws) % 16 != 0) return fail(TCAB_ERR_ALIGNMENT, "%s: the workspace is not 16-byte aligned", op);
+  return TCAB_OK;
+}
+uint64_t round256(uint64_t b) { return (b + 255) / 256 * 256; }
+
+__nv_bfloat16* bf16_of(const tcab_tensor* t) { return t != nullptr ? static_cast<__nv_bfloat16*>(t->data) : nullptr; }
+float* f32_of(const tcab_tensor* t) { return t != nullptr ? static_cast<float*>(t->data) : nullptr; }
+
 }  // namespace
 }  // namespace tcab
 
@@ -255,10 +366,12 @@ uint64_t tcab_launch_count(void) { return g_launches.load(std::memory_order_rela
 int tcab_device_status(int* status) {
   if (status == nullptr) return fail(TCAB_ERR_INVALID_ARG, "device_status: null output");
   TCAB_TRY(have_device("device_status"));
-  int gemm = 0, rows = 0;
+  int gemm = 0, rows = 0, ffn = 0;
   TCAB_TRY(gemm_device_status(&gemm));
   TCAB_TRY(rows_smem_status(&rows));
-  *status = gemm != 0 ? gemm : (rows != 0 ? 16 : 0);  // 1..4: a contraction kernel, 16: a shared-memory row kernel
+  TCAB_TRY(ffn_device_status(&ffn));
+  // 1..5: a kernel of gemm_bias_act.cu, 8: one of ffn_gemm.cuh, 16: a shared-memory row kernel
+  *status = gemm != 0 ? gemm : ffn != 0 ? 8 : (rows != 0 ? 16 : 0);
   return TCAB_OK;
 }
 
@@ -324,7 +437,7 @@ int prepare_common(const char* op, const tcab_chain* chain, const int32_t* in_dt
 }  // namespace
 
 int tcab_tune(const char* family, int p0, int p1, int p2, int p3) {
-  static const char* names[kFamilies] = {"softmax", "layernorm", "reduce_inner", "reduce_outer", "gemm"};
+  static const char* names[kFamilies] = {"softmax", "layernorm", "reduce_inner", "reduce_outer", "gemm", "ffn"};
   if (family == nullptr) return fail(TCAB_ERR_INVALID_ARG, "tune: null family");
   for (int i = 0; i < kFamilies; ++i) {
     if (std::strcmp(family, names[i]) == 0) {
@@ -423,9 +536,9 @@ int tcab_layernorm_rows(const tcab_tensor* x, const tcab_tensor* gamma, const tc
     return launch_layernorm_rows_bf16(static_cast<const __nv_bfloat16*>(x->data),
                                       static_cast<const __nv_bfloat16*>(gamma->data),
                                       static_cast<const __nv_bfloat16*>(beta->data), eps,
-                                      static_cast<__nv_bfloat16*>(y->data), rows, cols, s);
+                                      static_cast<__nv_bfloat16*>(y->data), RowStats{}, rows, cols, s);
   return launch_layernorm_rows_f32(static_cast<const float*>(x->data), static_cast<const float*>(gamma->data),
-                                   static_cast<const float*>(beta->data), eps, static_cast<float*>(y->data), rows,
+                                   static_cast<const float*>(beta->data), eps, static_cast<float*>(y->data), RowStats{}, rows,
                                    cols, s);
 }
 
@@ -697,6 +810,246 @@ int tcab_gemm_bias_act(const tcab_tensor* a, const tcab_tensor* b, const tcab_te
   return launch_gemm_bias_act(static_cast<const __nv_bfloat16*>(a->data), static_cast<const __nv_bfloat16*>(b->data),
                               bias ? static_cast<const float*>(bias->data) : nullptr, act,
                               static_cast<__nv_bfloat16*>(c->data), m, n, k, static_cast<cudaStream_t>(stream));
+}
+
+int tcab_layernorm_rows_stats(const tcab_tensor* x, const tcab_tensor* gamma, const tcab_tensor* beta, float eps,
+                              const tcab_tensor* y, const tcab_tensor* mean, const tcab_tensor* rstd, void* stream) {
+  const char* op = "layernorm_rows_stats";
+  TCAB_TRY(check_norm_rows(op, x));
+  const uint32_t cols = x->dims[x->rank - 1];
+  TCAB_TRY(check_like_x(op, "y", y, x));
+  TCAB_TRY(check_row_param(op, "gamma", gamma, cols, x->dtype, "the element type of x"));
+  TCAB_TRY(check_row_param(op, "beta", beta, cols, x->dtype, "the element type of x"));
+  TCAB_TRY(check_row_stats(op, "mean", mean, x));
+  TCAB_TRY(check_row_stats(op, "rstd", rstd, x));
+  const Named outs[] = {{"y", y}, {"mean", mean}, {"rstd", rstd}}, ins[] = {{"x", x}, {"gamma", gamma}, {"beta", beta}};
+  const tcab_tensor* may_be[] = {x};
+  TCAB_TRY(need_disjoint(op, outs, 3, ins, 3, may_be, 1));
+  TCAB_TRY(have_device(op));
+  const uint64_t rows = count(x, 0, x->rank - 1);
+  const RowStats st = {f32_of(mean), f32_of(rstd)};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (x->dtype == TCAB_BF16)
+    return launch_layernorm_rows_bf16(bf16_of(x), bf16_of(gamma), bf16_of(beta), eps, bf16_of(y), st, rows, cols, s);
+  return launch_layernorm_rows_f32(f32_of(x), f32_of(gamma), f32_of(beta), eps, f32_of(y), st, rows, cols, s);
+}
+
+uint64_t tcab_layernorm_rows_backward_workspace(const tcab_tensor* x) {
+  if (x == nullptr || x->rank < 1 || x->rank > TCAB_MAX_RANK || (x->dtype != TCAB_F32 && x->dtype != TCAB_BF16)) return 0;
+  const uint32_t cols = x->dims[x->rank - 1];
+  return cols == 0 ? 0 : layernorm_backward_workspace(count(x, 0, x->rank - 1), cols, x->dtype == TCAB_F32 ? 4 : 2);
+}
+
+int tcab_layernorm_rows_backward(const tcab_tensor* dy, const tcab_tensor* x, const tcab_tensor* gamma, const tcab_tensor* mean,
+                                 const tcab_tensor* rstd, const tcab_tensor* dx, const tcab_tensor* dgamma,
+                                 const tcab_tensor* dbeta, void* workspace, uint64_t workspace_bytes, void* stream) {
+  const char* op = "layernorm_rows_backward";
+  TCAB_TRY(check_norm_rows(op, x));
+  const uint32_t cols = x->dims[x->rank - 1];
+  TCAB_TRY(check_like_x(op, "dy", dy, x));
+  TCAB_TRY(check_like_x(op, "dx", dx, x));
+  TCAB_TRY(check_row_param(op, "gamma", gamma, cols, x->dtype, "the element type of x"));
+  TCAB_TRY(check_row_stats(op, "mean", mean, x));
+  TCAB_TRY(check_row_stats(op, "rstd", rstd, x));
+  TCAB_TRY(check_row_param(op, "dgamma", dgamma, cols, TCAB_F32, "f32"));
+  TCAB_TRY(check_row_param(op, "dbeta", dbeta, cols, TCAB_F32, "f32"));
+  const Named outs[] = {{"dx", dx}, {"dgamma", dgamma}, {"dbeta", dbeta}};
+  const Named ins[] = {{"dy", dy}, {"x", x}, {"gamma", gamma}, {"mean", mean}, {"rstd", rstd}};
+  const tcab_tensor* may_be[] = {dy, x};
+  TCAB_TRY(need_disjoint(op, outs, 3, ins, 5, may_be, 2));
+  TCAB_TRY(have_device(op));
+  TCAB_TRY(check_workspace(op, workspace, workspace_bytes, tcab_layernorm_rows_backward_workspace(x)));
+  const uint64_t rows = count(x, 0, x->rank - 1);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (x->dtype == TCAB_BF16)
+    return launch_layernorm_backward_bf16(bf16_of(dy), bf16_of(x), bf16_of(gamma), f32_of(mean), f32_of(rstd), bf16_of(dx),
+                                          f32_of(dgamma), f32_of(dbeta), rows, cols, workspace, workspace_bytes, s);
+  return launch_layernorm_backward_f32(f32_of(dy), f32_of(x), f32_of(gamma), f32_of(mean), f32_of(rstd), f32_of(dx),
+                                       f32_of(dgamma), f32_of(dbeta), rows, cols, workspace, workspace_bytes, s);
+}
+
+int tcab_gemm_bias_act_residual(const tcab_tensor* a, const tcab_tensor* b, const tcab_tensor* bias, const tcab_tensor* residual,
+                                int act, const tcab_tensor* preact, const tcab_tensor* c, void* stream) {
+  const char* op = "gemm_bias_act_residual";
+  uint32_t m = 0, k = 0, n = 0;
+  TCAB_TRY(check_contraction(op, "a", a, "b", b, &m, &k, &n));
+  TCAB_TRY(check_matrix(op, "c", c, m, n));
+  TCAB_TRY(check_matrix_opt(op, "residual", residual, m, n));
+  TCAB_TRY(check_matrix_opt(op, "preact", preact, m, n));
+  TCAB_TRY(check_bias_opt(op, "bias", bias, n));
+  if (act < TCAB_ACT_NONE || act > TCAB_ACT_GELU_TANH) return fail(TCAB_ERR_INVALID_ARG, "%s: unknown activation %d", op, act);
+  const Named outs[] = {{"c", c}, {"preact", preact}}, ins[] = {{"a", a}, {"b", b}, {"bias", bias}, {"residual", residual}};
+  const tcab_tensor* may_be[] = {residual};
+  TCAB_TRY(need_disjoint(op, outs, 2, ins, 4, may_be, residual != nullptr ? 1 : 0));
+  TCAB_TRY(have_device(op));
+  FfnProblem p;
+  p.a[0] = bf16_of(a);
+  p.b[0] = bf16_of(b);
+  p.c[0] = bf16_of(c);
+  p.z[0] = bf16_of(preact);
+  p.bias[0] = f32_of(bias);
+  p.residual = bf16_of(residual);
+  p.M = m;
+  p.N = n;
+  p.K = k;
+  p.act = act;
+  return launch_ffn_gemm(op, kFfnFwd, p, static_cast<cudaStream_t>(stream));
+}
+
+uint64_t tcab_gemm_bias_act_backward_workspace(uint32_t m, uint32_t n, int act, int with_dbias) {
+  const uint64_t dz = act == TCAB_ACT_NONE ? 0 : round256(2ull * m * n);
+  return dz + (with_dbias ? round256(act_backward_workspace(m, n, 0)) : 0);
+}
+
+int tcab_gemm_bias_act_backward(const tcab_tensor* dc, const tcab_tensor* a, const tcab_tensor* b, const tcab_tensor* preact,
+                                int act, const tcab_tensor* da, const tcab_tensor* db, const tcab_tensor* dbias,
+                                void* workspace, uint64_t workspace_bytes, void* stream) {
+  const char* op = "gemm_bias_act_backward";
+  uint32_t m = 0, k = 0, n = 0;
+  TCAB_TRY(check_contraction(op, "a", a, "b", b, &m, &k, &n));
+  TCAB_TRY(check_matrix(op, "dc", dc, m, n));
+  if (act < TCAB_ACT_NONE || act > TCAB_ACT_GELU_TANH) return fail(TCAB_ERR_INVALID_ARG, "%s: unknown activation %d", op, act);
+  if (act != TCAB_ACT_NONE && preact == nullptr)
+    return fail(TCAB_ERR_INVALID_ARG, "%s: preact is required for every activation but none", op);
+  TCAB_TRY(check_matrix_opt(op, "preact", preact, m, n));
+  TCAB_TRY(check_matrix_opt(op, "da", da, m, k));
+  TCAB_TRY(check_matrix_opt(op, "db", db, k, n));
+  TCAB_TRY(check_bias_opt(op, "dbias", dbias, n));
+  const Named outs[] = {{"da", da}, {"db", db}, {"dbias", dbias}}, ins[] = {{"dc", dc}, {"a", a}, {"b", b}, {"preact", preact}};
+  TCAB_TRY(need_disjoint(op, outs, 3, ins, 4));
+  TCAB_TRY(have_device(op));
+  TCAB_TRY(check_workspace(op, workspace, workspace_bytes, tcab_gemm_bias_act_backward_workspace(m, n, act, dbias != nullptr)));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const __nv_bfloat16* dz = bf16_of(dc);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const bool contract = da != nullptr || db != nullptr;
+  if (act != TCAB_ACT_NONE && (contract || dbias != nullptr)) {
+    __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(ws);
+    TCAB_TRY(launch_act_backward(op, act, dz, bf16_of(preact), contract ? to : nullptr, f32_of(dbias), m, n, ws + round256(2ull * m * n), s));
+    dz = to;
+  } else if (dbias != nullptr) {
+    TCAB_TRY(launch_act_backward(op, TCAB_ACT_NONE, dz, nullptr, nullptr, f32_of(dbias), m, n, ws, s));
+  }
+  if (da != nullptr) {
+    FfnProblem p;
+    p.a[0] = dz;
+    p.b[0] = bf16_of(b);
+    p.c[0] = bf16_of(da);
+    p.M = m;
+    p.N = k;
+    p.K = n;
+    TCAB_TRY(launch_ffn_gemm(op, kFfnDx, p, s));
+  }
+  if (db != nullptr) {
+    FfnProblem p;
+    p.a[0] = bf16_of(a);
+    p.b[0] = dz;
+    p.c[0] = bf16_of(db);
+    p.M = k;
+    p.N = n;
+    p.K = m;
+    TCAB_TRY(launch_ffn_gemm(op, kFfnDw, p, s));
+  }
+  return TCAB_OK;
+}
+
+int tcab_gated_gemm(const tcab_tensor* x, const tcab_tensor* w_gate, const tcab_tensor* w_up, const tcab_tensor* bias_gate,
+                    const tcab_tensor* bias_up, int act, const tcab_tensor* gate, const tcab_tensor* up, const tcab_tensor* h,
+                    void* stream) {
+  const char* op = "gated_gemm";
+  uint32_t m = 0, k = 0, n = 0;
+  TCAB_TRY(check_contraction(op, "x", x, "w_gate", w_gate, &m, &k, &n));
+  TCAB_TRY(check_matrix(op, "w_up", w_up, k, n));
+  TCAB_TRY(check_matrix(op, "h", h, m, n));
+  if ((gate == nullptr) != (up == nullptr)) return fail(TCAB_ERR_INVALID_ARG, "%s: gate and up are stored both or neither", op);
+  if ((bias_gate == nullptr) != (bias_up == nullptr)) return fail(TCAB_ERR_INVALID_ARG, "%s: bias_gate and bias_up come both or neither", op);
+  TCAB_TRY(check_matrix_opt(op, "gate", gate, m, n));
+  TCAB_TRY(check_matrix_opt(op, "up", up, m, n));
+  TCAB_TRY(check_bias_opt(op, "bias_gate", bias_gate, n));
+  TCAB_TRY(check_bias_opt(op, "bias_up", bias_up, n));
+  if (act < TCAB_ACT_RELU || act > TCAB_ACT_SIGMOID) return fail(TCAB_ERR_INVALID_ARG, "%s: unknown activation %d", op, act);
+  const Named outs[] = {{"h", h}, {"gate", gate}, {"up", up}};
+  const Named ins[] = {{"x", x}, {"w_gate", w_gate}, {"w_up", w_up}, {"bias_gate", bias_gate}, {"bias_up", bias_up}};
+  TCAB_TRY(need_disjoint(op, outs, 3, ins, 5));
+  TCAB_TRY(have_device(op));
+  FfnProblem p;
+  p.a[0] = bf16_of(x);
+  p.b[0] = bf16_of(w_gate);
+  p.b[1] = bf16_of(w_up);
+  p.c[0] = bf16_of(h);
+  p.z[0] = bf16_of(gate);
+  p.z[1] = bf16_of(up);
+  p.bias[0] = f32_of(bias_gate);
+  p.bias[1] = f32_of(bias_up);
+  p.M = m;
+  p.N = n;
+  p.K = k;
+  p.act = act;
+  return launch_ffn_gemm(op, kFfnGated, p, static_cast<cudaStream_t>(stream));
+}
+
+uint64_t tcab_gated_gemm_backward_workspace(uint32_t m, uint32_t n, int with_dbias) {
+  return 2 * round256(2ull * m * n) + (with_dbias ? round256(act_backward_workspace(m, n, 1)) : 0);
+}
+
+int tcab_gated_gemm_backward(const tcab_tensor* dh, const tcab_tensor* x, const tcab_tensor* w_gate, const tcab_tensor* w_up,
+                             const tcab_tensor* gate, const tcab_tensor* up, int act, const tcab_tensor* dx,
+                             const tcab_tensor* dw_gate, const tcab_tensor* dw_up, const tcab_tensor* dbias_gate,
+                             const tcab_tensor* dbias_up, void* workspace, uint64_t workspace_bytes, void* stream) {
+  const char* op = "gated_gemm_backward";
+  uint32_t m = 0, k = 0, n = 0;
+  TCAB_TRY(check_contraction(op, "x", x, "w_gate", w_gate, &m, &k, &n));
+  TCAB_TRY(check_matrix(op, "w_up", w_up, k, n));
+  TCAB_TRY(check_matrix(op, "dh", dh, m, n));
+  TCAB_TRY(check_matrix(op, "gate", gate, m, n));
+  TCAB_TRY(check_matrix(op, "up", up, m, n));
+  if (act < TCAB_ACT_RELU || act > TCAB_ACT_SIGMOID) return fail(TCAB_ERR_INVALID_ARG, "%s: unknown activation %d", op, act);
+  if ((dw_gate == nullptr) != (dw_up == nullptr)) return fail(TCAB_ERR_INVALID_ARG, "%s: dw_gate and dw_up come both or neither", op);
+  if ((dbias_gate == nullptr) != (dbias_up == nullptr))
+    return fail(TCAB_ERR_INVALID_ARG, "%s: dbias_gate and dbias_up come both or neither", op);
+  TCAB_TRY(check_matrix_opt(op, "dx", dx, m, k));
+  TCAB_TRY(check_matrix_opt(op, "dw_gate", dw_gate, k, n));
+  TCAB_TRY(check_matrix_opt(op, "dw_up", dw_up, k, n));
+  TCAB_TRY(check_bias_opt(op, "dbias_gate", dbias_gate, n));
+  TCAB_TRY(check_bias_opt(op, "dbias_up", dbias_up, n));
+  const Named outs[] = {{"dx", dx}, {"dw_gate", dw_gate}, {"dw_up", dw_up}, {"dbias_gate", dbias_gate}, {"dbias_up", dbias_up}};
+  const Named ins[] = {{"dh", dh}, {"x", x}, {"w_gate", w_gate}, {"w_up", w_up}, {"gate", gate}, {"up", up}};
+  TCAB_TRY(need_disjoint(op, outs, 5, ins, 6));
+  TCAB_TRY(have_device(op));
+  TCAB_TRY(check_workspace(op, workspace, workspace_bytes, tcab_gated_gemm_backward_workspace(m, n, dbias_gate != nullptr)));
+  if (dx == nullptr && dw_gate == nullptr && dbias_gate == nullptr) return TCAB_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const uint64_t plane = round256(2ull * m * n);
+  __nv_bfloat16* dgate = reinterpret_cast<__nv_bfloat16*>(ws);
+  __nv_bfloat16* dup = reinterpret_cast<__nv_bfloat16*>(ws + plane);
+  TCAB_TRY(launch_gated_backward(op, act, bf16_of(dh), bf16_of(gate), bf16_of(up), dgate, dup, f32_of(dbias_gate), f32_of(dbias_up),
+                                 m, n, ws + 2 * plane, s));
+  if (dx != nullptr) {
+    FfnProblem p;
+    p.a[0] = dgate;
+    p.a[1] = dup;
+    p.b[0] = bf16_of(w_gate);
+    p.b[1] = bf16_of(w_up);
+    p.c[0] = bf16_of(dx);
+    p.M = m;
+    p.N = k;
+    p.K = n;
+    TCAB_TRY(launch_ffn_gemm(op, kFfnDx, p, s));
+  }
+  if (dw_gate != nullptr) {
+    FfnProblem p;
+    p.a[0] = bf16_of(x);
+    p.b[0] = dgate;
+    p.b[1] = dup;
+    p.c[0] = bf16_of(dw_gate);
+    p.c[1] = bf16_of(dw_up);
+    p.M = k;
+    p.N = n;
+    p.K = m;
+    TCAB_TRY(launch_ffn_gemm(op, kFfnDw, p, s));
+  }
+  return TCAB_OK;
 }
 
 }  // extern "C"

@@ -33,7 +33,7 @@ struct Tune {
   int p0 = 0, p1 = 0, p2 = 0, p3 = 0;
 };
 const Tune& tune(int family);
-enum Family { kSoftmax = 0, kLayernorm = 1, kReduceInner = 2, kReduceOuter = 3, kGemm = 4, kFamilies = 5 };
+enum Family { kSoftmax = 0, kLayernorm = 1, kReduceInner = 2, kReduceOuter = 3, kGemm = 4, kFfn = 5, kFamilies = 6 };
 
 // Resident CTAs per SM of a kernel at a block size / dynamic smem, cached per (function, block).
 int occupancy(const void* fn, int block, size_t smem);
@@ -47,6 +47,12 @@ int occupancy(const void* fn, int block, size_t smem);
 enum ScratchKind { kScratchChainSplit = 0, kScratchOuter = 1, kScratchGemm = 2, kScratchGemmCounters = 3, kScratchSplit3 = 4, kScratchKinds = 5 };
 void* stream_scratch(int kind, cudaStream_t stream, size_t bytes, bool grow, bool zero = false);
 
+#define TCAB_TRY_RC(expr)          \
+  do {                             \
+    const int tcab_rc2_ = (expr);  \
+    if (tcab_rc2_ != TCAB_OK) return tcab_rc2_; \
+  } while (0)
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 inline uint32_t pow2_ceil(uint32_t v) {
@@ -55,6 +61,19 @@ inline uint32_t pow2_ceil(uint32_t v) {
   return p;
 }
 
+// Where a layer-norm forward leaves a row's statistics for the backward pass; null pointers: nowhere.
+struct RowStats {
+  float* mean = nullptr;
+  float* rstd = nullptr;
+#ifdef __CUDACC__
+  __device__ __forceinline__ void put(uint64_t row, float m, float r) const {
+    if (mean == nullptr) return;
+    mean[row] = m;
+    rstd[row] = r;
+  }
+#endif
+};
+
 // Entry points of the operator classes (one .cu each).
 int launch_softmax_rows(const float* x, float* y, uint64_t rows, uint32_t cols, cudaStream_t s);
 // long rows held in shared memory (rows_smem.cu); the caller has checked 16-byte vectors and rows_smem_fits
@@ -62,14 +81,22 @@ bool rows_smem_fits(uint64_t row_bytes);
 int rows_smem_status(int* out);
 int launch_softmax_rows_smem(const float* x, float* y, uint64_t rows, uint32_t cols, cudaStream_t s);
 int launch_layernorm_rows_smem_bf16(const __nv_bfloat16* x, const __nv_bfloat16* gamma, const __nv_bfloat16* beta,
-                                    float eps, __nv_bfloat16* y, uint64_t rows, uint32_t cols, cudaStream_t s);
-int launch_layernorm_rows_smem_f32(const float* x, const float* gamma, const float* beta, float eps, float* y,
+                                    float eps, __nv_bfloat16* y, RowStats st, uint64_t rows, uint32_t cols, cudaStream_t s);
+int launch_layernorm_rows_smem_f32(const float* x, const float* gamma, const float* beta, float eps, float* y, RowStats st,
                                    uint64_t rows, uint32_t cols, cudaStream_t s);
 int launch_layernorm_rows_bf16(const __nv_bfloat16* x, const __nv_bfloat16* gamma,
-                               const __nv_bfloat16* beta, float eps, __nv_bfloat16* y,
+                               const __nv_bfloat16* beta, float eps, __nv_bfloat16* y, RowStats st,
                                uint64_t rows, uint32_t cols, cudaStream_t s);
 int launch_layernorm_rows_f32(const float* x, const float* gamma, const float* beta, float eps,
-                              float* y, uint64_t rows, uint32_t cols, cudaStream_t s);
+                              float* y, RowStats st, uint64_t rows, uint32_t cols, cudaStream_t s);
+// layernorm_backward.cu; the workspace of a size covers every alignment of its operands
+uint64_t layernorm_backward_workspace(uint64_t rows, uint32_t cols, int elem_bytes);
+int launch_layernorm_backward_bf16(const __nv_bfloat16* dy, const __nv_bfloat16* x, const __nv_bfloat16* gamma, const float* mean,
+                                   const float* rstd, __nv_bfloat16* dx, float* dgamma, float* dbeta, uint64_t rows, uint32_t cols,
+                                   void* ws, uint64_t ws_bytes, cudaStream_t s);
+int launch_layernorm_backward_f32(const float* dy, const float* x, const float* gamma, const float* mean, const float* rstd,
+                                  float* dx, float* dgamma, float* dbeta, uint64_t rows, uint32_t cols, void* ws,
+                                  uint64_t ws_bytes, cudaStream_t s);
 int launch_reduce_outer(const float* t, float* sum, float* mx, int32_t* amax, uint32_t nb,
                         uint32_t nk, uint32_t nc, cudaStream_t s);
 // What the run-time compiler needs to know about a chain: which kernels ('R' the reduction kernels, 'B' the

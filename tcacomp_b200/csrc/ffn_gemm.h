@@ -1,0 +1,47 @@
+// ffn_gemm.h -- the contractions of a feed-forward layer and of its backward pass (ffn_gemm.cuh), as their callers see them.
+#pragma once
+
+#include <cuda.h>
+
+#include "common.cuh"
+
+namespace tcab {
+
+enum FfnForm {
+  kFfnFwd = 0,    // c = act(a @ b + bias) + residual            a [M, K], b [K, N]
+  kFfnGated = 1,  // c = act(a @ b0 + bias0) * (a @ b1 + bias1)  a [M, K], b0, b1 [K, N]
+  kFfnDx = 2,     // c = a0 @ b0^T (+ a1 @ b1^T)                 a0, a1 [M, K], b0, b1 [N, K]
+  kFfnDw = 3      // c0 = a^T @ b0 (, c1 = a^T @ b1)             a [K, M], b0, b1 [K, N]
+};
+
+// One contraction. M, N: the extents of an output, K: the contracted one. Pointers are 16-byte aligned, the innermost
+// extents of every operand multiples of eight; any extent may be zero.
+struct FfnProblem {
+  const __nv_bfloat16* a[2] = {nullptr, nullptr};
+  const __nv_bfloat16* b[2] = {nullptr, nullptr};
+  __nv_bfloat16* c[2] = {nullptr, nullptr};
+  __nv_bfloat16* z[2] = {nullptr, nullptr};  // kFfnFwd: a @ b + bias, kFfnGated: both projections with their biases; or null
+  const float* bias[2] = {nullptr, nullptr};
+  const __nv_bfloat16* residual = nullptr;
+  uint32_t M = 0, N = 0, K = 0;
+  int act = TCAB_ACT_NONE;
+};
+
+int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t s);
+int ffn_device_status(int* out);
+
+// dz = dc * act'(z) (gated: dgate = dh * up * act'(gate), dup = dh * act(gate)), with the column sums of each where
+// wanted (act_backward.cu). dz may be null (column sums alone; act none). Partials of the sums go to `ws`.
+uint64_t act_backward_workspace(uint32_t rows, uint32_t cols, int gated);
+int launch_act_backward(const char* op, int act, const __nv_bfloat16* dc, const __nv_bfloat16* z, __nv_bfloat16* dz,
+                        float* dbias, uint32_t rows, uint32_t cols, void* ws, cudaStream_t s);
+int launch_gated_backward(const char* op, int act, const __nv_bfloat16* dh, const __nv_bfloat16* gate, const __nv_bfloat16* up,
+                          __nv_bfloat16* dgate, __nv_bfloat16* dup, float* dbias_gate, float* dbias_up, uint32_t rows,
+                          uint32_t cols, void* ws, cudaStream_t s);
+
+// A 2-D bf16 row-major tensor as a TMA tensor map (gemm_bias_act.cu): boxes of 64 columns (128-byte swizzle) or 32
+// columns (64-byte swizzle).
+int make_tensor_map(const char* op, CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
+                    uint32_t box_cols);
+
+}  // namespace tcab

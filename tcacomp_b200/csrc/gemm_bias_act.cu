@@ -35,6 +35,7 @@
 #include <utility>
 
 #include "common.cuh"
+#include "ffn_gemm.h"
 #include "sm100_ptx.cuh"
 
 namespace tcab {
@@ -1203,6 +1204,12 @@ int make_map_f32(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols,
 
 }  // namespace
 
+int make_tensor_map(const char* op, CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
+                    uint32_t box_cols) {
+  const int rc = make_map(m, base, rows, cols, box_rows, box_cols);
+  return rc == TCAB_OK ? rc : fail(rc, "%s: cannot describe a tensor of %llu x %llu to the copy engine", op,
+                                   static_cast<unsigned long long>(rows), static_cast<unsigned long long>(cols));
+}
 
 int gemm_device_status(int* out) {
   if (cudaMemcpyFromSymbol(out, g_gemm_status, sizeof(int)) != cudaSuccess) {

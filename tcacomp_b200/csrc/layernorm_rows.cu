@@ -9,6 +9,9 @@
 // runner testing/runners/layernorm.cu:47-58). bf16 rows are widened to fp32 on
 // load and rounded to nearest even on store (design/syntax-design.md:601-607).
 //
+// Every kernel can also store a row's mean and 1 / sqrtf(var + eps) (RowStats: what the backward pass reads instead
+// of taking the statistics again, 8 bytes per row); the stored rows are the same bits either way.
+//
 // The row lives in registers, so x is read once and y written once (4 bytes per
 // bf16 element, 8 per fp32 element: the roofline figure). gamma and beta are either re-read per row through the read-only
 // L1 path (they total a few KB and stay L1-resident; the row itself streams past
@@ -23,7 +26,7 @@ namespace {
 template <typename T, int TPR, int VPT, int V, bool CACHE_GB>
 __global__ void __launch_bounds__(row_cta_threads(TPR), CACHE_GB ? 1 : row_min_ctas(TPR, VPT * V, sizeof(T) == 2 ? 32 : 16, TPR == 512 ? 1536 : TPR == 1024 ? 2048 : 1280))
 layernorm_rows_reg(const T* __restrict__ x, const T* __restrict__ gamma, const T* __restrict__ beta,
-                   float eps, T* __restrict__ y, uint64_t rows, uint32_t cols) {
+                   float eps, T* __restrict__ y, RowStats st, uint64_t rows, uint32_t cols) {
   constexpr int THREADS = row_cta_threads(TPR);
   constexpr int GROUPS = THREADS / TPR;
   using IO = VecIO<T, V>;
@@ -92,6 +95,7 @@ layernorm_rows_reg(const T* __restrict__ x, const T* __restrict__ gamma, const T
     }
     q = group_allreduce<OpSum, TPR>(q, slots[1], g);
     const float rstd = 1.0f / sqrtf(q / n + eps);
+    if (live && t == 0) st.put(row, mean, rstd);
 
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -215,7 +219,7 @@ constexpr int unaligned_threads_per_sm(int tpr, int vpt) {
 template <typename T, int TPR, int VPT>
 __global__ void __launch_bounds__(row_cta_threads(TPR), unaligned_threads_per_sm<T>(TPR, VPT) / row_cta_threads(TPR))
 layernorm_rows_reg_unaligned(const T* __restrict__ x, const T* __restrict__ gamma, const T* __restrict__ beta,
-                             float eps, T* __restrict__ y, uint64_t rows, uint32_t cols) {
+                             float eps, T* __restrict__ y, RowStats st, uint64_t rows, uint32_t cols) {
   constexpr int THREADS = row_cta_threads(TPR);
   constexpr int GROUPS = THREADS / TPR;
   constexpr int V = 16 / sizeof(T);
@@ -274,6 +278,7 @@ layernorm_rows_reg_unaligned(const T* __restrict__ x, const T* __restrict__ gamm
     }
     q = group_allreduce<OpSum, TPR>(q, slots[1], g);
     const float rstd = 1.0f / sqrtf(q / n + eps);
+    if (live && t == 0) st.put(row, mean, rstd);
 
     if (ec >= 0) {
       float gf, bf;
@@ -298,13 +303,13 @@ layernorm_rows_reg_unaligned(const T* __restrict__ x, const T* __restrict__ gamm
 }
 
 template <typename T, int TPR, int VPT>
-int launch_reg_unaligned(const T* x, const T* gamma, const T* beta, float eps, T* y, uint64_t rows, uint32_t cols,
+int launch_reg_unaligned(const T* x, const T* gamma, const T* beta, float eps, T* y, RowStats st, uint64_t rows, uint32_t cols,
                          cudaStream_t s) {
   constexpr int THREADS = row_cta_threads(TPR);
   constexpr int GROUPS = THREADS / TPR;
   uint64_t grid = (rows + GROUPS - 1) / GROUPS;
   if (grid > 0x7fffffffull) grid = 0x7fffffffull;
-  layernorm_rows_reg_unaligned<T, TPR, VPT><<<static_cast<unsigned>(grid), THREADS, 0, s>>>(x, gamma, beta, eps, y, rows, cols);
+  layernorm_rows_reg_unaligned<T, TPR, VPT><<<static_cast<unsigned>(grid), THREADS, 0, s>>>(x, gamma, beta, eps, y, st, rows, cols);
   count_launch();
   return check_launch("layernorm_rows_reg_unaligned");
 }
@@ -314,7 +319,7 @@ int launch_reg_unaligned(const T* x, const T* gamma, const T* beta, float eps, T
 template <typename T, int THREADS, int VPT, int V>
 __global__ void __launch_bounds__(THREADS)
 layernorm_rows_cluster(const T* __restrict__ x, const T* __restrict__ gamma, const T* __restrict__ beta, float eps,
-                       T* __restrict__ y, uint32_t cols, uint32_t cs, uint32_t seg_vecs) {
+                       T* __restrict__ y, RowStats st, uint32_t cols, uint32_t cs, uint32_t seg_vecs) {
   using IO = VecIO<T, V>;
   __shared__ float slots[2][32];
   __shared__ float cl_sum, cl_sq;
@@ -368,6 +373,7 @@ layernorm_rows_cluster(const T* __restrict__ x, const T* __restrict__ gamma, con
   float gq = 0.0f;
   for (uint32_t r = 0; r < cs; ++r) gq += ld_dsmem(&cl_sq, r);
   const float rstd = 1.0f / sqrtf(gq / n + eps);
+  if (rank == 0 && threadIdx.x == 0) st.put(row, mean, rstd);
 
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
@@ -385,7 +391,7 @@ layernorm_rows_cluster(const T* __restrict__ x, const T* __restrict__ gamma, con
 }
 
 template <typename T, int THREADS, int VPT, int V>
-int launch_cluster_shape(const T* x, const T* gamma, const T* beta, float eps, T* y, uint64_t rows, uint32_t cols,
+int launch_cluster_shape(const T* x, const T* gamma, const T* beta, float eps, T* y, RowStats st, uint64_t rows, uint32_t cols,
                          uint32_t nvec, cudaStream_t s) {
   constexpr uint32_t kPerCta = THREADS * VPT;
   // the smallest cluster (2..8 CTAs, any size) whose CTAs cover the row
@@ -405,7 +411,7 @@ int launch_cluster_shape(const T* x, const T* gamma, const T* beta, float eps, T
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, x, gamma, beta, eps, y, cols, cs, seg);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, x, gamma, beta, eps, y, st, cols, cs, seg);
   count_launch();
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -415,14 +421,14 @@ int launch_cluster_shape(const T* x, const T* gamma, const T* beta, float eps, T
 }
 
 template <typename T, int V>
-int launch_cluster(const T* x, const T* gamma, const T* beta, float eps, T* y, uint64_t rows, uint32_t cols,
+int launch_cluster(const T* x, const T* gamma, const T* beta, float eps, T* y, RowStats st, uint64_t rows, uint32_t cols,
                    uint32_t nvec, cudaStream_t s) {
   const Tune& tn = tune(kLayernorm);
   // 512 threads x 8 vectors per CTA; the 256-thread shapes (tune p2 = 4 / 8 vectors per thread, for sweeps)
   // measured slower for layer-norm
-  if (tn.p2 == 4 && nvec <= 8u * 256u * 4u) return launch_cluster_shape<T, 256, 4, V>(x, gamma, beta, eps, y, rows, cols, nvec, s);
-  if (tn.p2 == 8 && nvec <= 8u * 256u * 8u) return launch_cluster_shape<T, 256, 8, V>(x, gamma, beta, eps, y, rows, cols, nvec, s);
-  return launch_cluster_shape<T, 512, 8, V>(x, gamma, beta, eps, y, rows, cols, nvec, s);
+  if (tn.p2 == 4 && nvec <= 8u * 256u * 4u) return launch_cluster_shape<T, 256, 4, V>(x, gamma, beta, eps, y, st, rows, cols, nvec, s);
+  if (tn.p2 == 8 && nvec <= 8u * 256u * 8u) return launch_cluster_shape<T, 256, 8, V>(x, gamma, beta, eps, y, st, rows, cols, nvec, s);
+  return launch_cluster_shape<T, 512, 8, V>(x, gamma, beta, eps, y, st, rows, cols, nvec, s);
 }
 
 // Long rows streamed by a cluster (the scheme of softmax_rows_cluster_stream): one segment per CTA, nothing kept
@@ -434,7 +440,7 @@ int launch_cluster(const T* x, const T* gamma, const T* beta, float eps, T* y, u
 template <typename T, int THREADS, int U, int V>
 __global__ void __launch_bounds__(THREADS)
 layernorm_rows_cluster_stream(const T* __restrict__ x, const T* __restrict__ gamma, const T* __restrict__ beta,
-                              float eps, T* __restrict__ y, uint32_t cols, uint32_t cs, uint32_t seg_vecs) {
+                              float eps, T* __restrict__ y, RowStats st, uint32_t cols, uint32_t cs, uint32_t seg_vecs) {
   using IO = VecIO<T, V>;
   __shared__ float slots[2][32];
   __shared__ float cl_a[2], cl_b;  // this CTA's partials, read by the whole cluster
@@ -514,6 +520,7 @@ layernorm_rows_cluster_stream(const T* __restrict__ x, const T* __restrict__ gam
     var = gq / n;
   }
   const float rstd = 1.0f / sqrtf(var + eps);
+  if (rank == 0 && threadIdx.x == 0) st.put(row, mean, rstd);
   for (uint32_t base = v0 + threadIdx.x; base < v1; base += THREADS * U) {
     float f[U][V];
 #pragma unroll
@@ -538,7 +545,7 @@ layernorm_rows_cluster_stream(const T* __restrict__ x, const T* __restrict__ gam
 }
 
 template <typename T, int THREADS, int U, int V>
-int launch_cluster_stream_shape(const T* x, const T* gamma, const T* beta, float eps, T* y, uint64_t rows, uint32_t cols,
+int launch_cluster_stream_shape(const T* x, const T* gamma, const T* beta, float eps, T* y, RowStats st, uint64_t rows, uint32_t cols,
                                 uint32_t nvec, uint32_t cs, cudaStream_t s) {
   const uint32_t seg = (nvec + cs - 1) / cs;
   auto* fn = layernorm_rows_cluster_stream<T, THREADS, U, V>;
@@ -553,7 +560,7 @@ int launch_cluster_stream_shape(const T* x, const T* gamma, const T* beta, float
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, x, gamma, beta, eps, y, cols, cs, seg);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, x, gamma, beta, eps, y, st, cols, cs, seg);
   count_launch();
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -564,7 +571,7 @@ int launch_cluster_stream_shape(const T* x, const T* gamma, const T* beta, float
 
 // tune("layernorm", _, p1 = CTAs per row, p2 = shape 1..5, p3 = 7) forces a shape of the streaming clusters.
 template <typename T, int V>
-int launch_cluster_stream(const T* x, const T* gamma, const T* beta, float eps, T* y, uint64_t rows, uint32_t cols,
+int launch_cluster_stream(const T* x, const T* gamma, const T* beta, float eps, T* y, RowStats st, uint64_t rows, uint32_t cols,
                           uint32_t nvec, bool few_rows, cudaStream_t s) {
   const Tune& tn = tune(kLayernorm);
   uint32_t cs = 0;
@@ -580,11 +587,11 @@ int launch_cluster_stream(const T* x, const T* gamma, const T* beta, float eps, 
   if (shape <= 0) shape = nvec <= 8u * 1024u * 4u ? 1 : nvec <= 8u * 2048u * 4u ? 2 : 5;
   if (cs == 0) cs = stream_cluster_size(nvec, shape == 1 ? 1024u : shape == 5 ? 4096u : 2048u, sizeof(T) == 4);
   switch (shape) {
-    case 1: return launch_cluster_stream_shape<T, 256, 4, V>(x, gamma, beta, eps, y, rows, cols, nvec, cs, s);
-    case 2: return launch_cluster_stream_shape<T, 512, 4, V>(x, gamma, beta, eps, y, rows, cols, nvec, cs, s);
-    case 3: return launch_cluster_stream_shape<T, 256, 8, V>(x, gamma, beta, eps, y, rows, cols, nvec, cs, s);
-    case 4: return launch_cluster_stream_shape<T, 256, 2, V>(x, gamma, beta, eps, y, rows, cols, nvec, cs, s);
-    default: return launch_cluster_stream_shape<T, 512, 8, V>(x, gamma, beta, eps, y, rows, cols, nvec, cs, s);
+    case 1: return launch_cluster_stream_shape<T, 256, 4, V>(x, gamma, beta, eps, y, st, rows, cols, nvec, cs, s);
+    case 2: return launch_cluster_stream_shape<T, 512, 4, V>(x, gamma, beta, eps, y, st, rows, cols, nvec, cs, s);
+    case 3: return launch_cluster_stream_shape<T, 256, 8, V>(x, gamma, beta, eps, y, st, rows, cols, nvec, cs, s);
+    case 4: return launch_cluster_stream_shape<T, 256, 2, V>(x, gamma, beta, eps, y, st, rows, cols, nvec, cs, s);
+    default: return launch_cluster_stream_shape<T, 512, 8, V>(x, gamma, beta, eps, y, st, rows, cols, nvec, cs, s);
   }
 }
 
@@ -593,7 +600,7 @@ int launch_cluster_stream(const T* x, const T* gamma, const T* beta, float eps, 
 template <typename T, int THREADS, int V>
 __global__ void __launch_bounds__(THREADS)
 layernorm_rows_stream(const T* __restrict__ x, const T* __restrict__ gamma, const T* __restrict__ beta,
-                      float eps, T* __restrict__ y, uint64_t rows, uint32_t cols) {
+                      float eps, T* __restrict__ y, RowStats st, uint64_t rows, uint32_t cols) {
   using IO = VecIO<T, V>;
   __shared__ float slots[2][32];
   const uint32_t nvec = cols / V;
@@ -617,6 +624,7 @@ layernorm_rows_stream(const T* __restrict__ x, const T* __restrict__ gamma, cons
       for (int j = 0; j < V; ++j) q += (f[j] - mean) * (f[j] - mean);
     }
     const float rstd = 1.0f / sqrtf(cta_allreduce<OpSum, THREADS / 32>(q, slots[1]) / n + eps);
+    if (threadIdx.x == 0) st.put(row, mean, rstd);
     for (uint32_t idx = threadIdx.x; idx < nvec; idx += THREADS) {
       float f[V], gf[V], bf[V];
       IO::unpack(IO::load(xr, idx), f);
@@ -631,7 +639,7 @@ layernorm_rows_stream(const T* __restrict__ x, const T* __restrict__ gamma, cons
 }
 
 template <typename T, int TPR, int VPT, int V, bool CACHE_GB>
-int launch_reg2(const T* x, const T* gamma, const T* beta, float eps, T* y, uint64_t rows, uint32_t cols,
+int launch_reg2(const T* x, const T* gamma, const T* beta, float eps, T* y, RowStats st, uint64_t rows, uint32_t cols,
                 int ctas_per_sm, cudaStream_t s) {
   constexpr int THREADS = row_cta_threads(TPR);
   constexpr int GROUPS = THREADS / TPR;
@@ -642,18 +650,18 @@ int launch_reg2(const T* x, const T* gamma, const T* beta, float eps, T* y, uint
   uint64_t grid = ctas_per_sm > 0 ? static_cast<uint64_t>(sm_count()) * ctas_per_sm : need;
   if (grid > need) grid = need;
   if (grid > 0x7fffffffull) grid = 0x7fffffffull;
-  fn<<<static_cast<unsigned>(grid), THREADS, 0, s>>>(x, gamma, beta, eps, y, rows, cols);
+  fn<<<static_cast<unsigned>(grid), THREADS, 0, s>>>(x, gamma, beta, eps, y, st, rows, cols);
   count_launch();
   return check_launch("layernorm_rows_reg");
 }
 
 // tune p3 == 1 selects the register-cached gamma/beta variant.
 template <typename T, int TPR, int VPT, int V>
-int launch_reg(const T* x, const T* gamma, const T* beta, float eps, T* y, uint64_t rows, uint32_t cols,
+int launch_reg(const T* x, const T* gamma, const T* beta, float eps, T* y, RowStats st, uint64_t rows, uint32_t cols,
                int ctas_per_sm, cudaStream_t s) {
   if (tune(kLayernorm).p3 == 1)
-    return launch_reg2<T, TPR, VPT, V, true>(x, gamma, beta, eps, y, rows, cols, ctas_per_sm, s);
-  return launch_reg2<T, TPR, VPT, V, false>(x, gamma, beta, eps, y, rows, cols, ctas_per_sm, s);
+    return launch_reg2<T, TPR, VPT, V, true>(x, gamma, beta, eps, y, st, rows, cols, ctas_per_sm, s);
+  return launch_reg2<T, TPR, VPT, V, false>(x, gamma, beta, eps, y, st, rows, cols, ctas_per_sm, s);
 }
 
 #define TCAB_LN_SHAPES_BASE(X) \
@@ -664,16 +672,16 @@ int launch_reg(const T* x, const T* gamma, const T* beta, float eps, T* y, uint6
   X(16, 5) X(32, 5) X(64, 5) X(128, 5) X(256, 5) X(16, 3) X(32, 3) X(64, 3) X(128, 3) X(256, 3) X(512, 3)
 
 inline int launch_smem(const __nv_bfloat16* x, const __nv_bfloat16* gamma, const __nv_bfloat16* beta, float eps,
-                       __nv_bfloat16* y, uint64_t rows, uint32_t cols, cudaStream_t s) {
-  return launch_layernorm_rows_smem_bf16(x, gamma, beta, eps, y, rows, cols, s);
+                       __nv_bfloat16* y, RowStats st, uint64_t rows, uint32_t cols, cudaStream_t s) {
+  return launch_layernorm_rows_smem_bf16(x, gamma, beta, eps, y, st, rows, cols, s);
 }
-inline int launch_smem(const float* x, const float* gamma, const float* beta, float eps, float* y, uint64_t rows,
+inline int launch_smem(const float* x, const float* gamma, const float* beta, float eps, float* y, RowStats st, uint64_t rows,
                        uint32_t cols, cudaStream_t s) {
-  return launch_layernorm_rows_smem_f32(x, gamma, beta, eps, y, rows, cols, s);
+  return launch_layernorm_rows_smem_f32(x, gamma, beta, eps, y, st, rows, cols, s);
 }
 
 template <typename T, int VW>
-int dispatch(const T* x, const T* gamma, const T* beta, float eps, T* y, uint64_t rows, uint32_t cols,
+int dispatch(const T* x, const T* gamma, const T* beta, float eps, T* y, RowStats st, uint64_t rows, uint32_t cols,
              cudaStream_t s) {
   if (rows == 0 || cols == 0) return TCAB_OK;
   const bool vec = (cols % VW == 0) && aligned16(x) && aligned16(y) && aligned16(gamma) && aligned16(beta);
@@ -686,7 +694,7 @@ int dispatch(const T* x, const T* gamma, const T* beta, float eps, T* y, uint64_
     if (choose_row_shape_fit(cols / VW, true, true, VW, &ut, &uv) && ut >= 2 * (VW - 1)) {
 #define TCAB_CASE(TP, P) \
   if constexpr (TP >= 2 * (VW - 1) && (TP < 1024 || P * VW <= 32)) /* longer rows would spill */ \
-    if (ut == TP && uv == P) return launch_reg_unaligned<T, TP, P>(x, gamma, beta, eps, y, rows, cols, s);
+    if (ut == TP && uv == P) return launch_reg_unaligned<T, TP, P>(x, gamma, beta, eps, y, st, rows, cols, s);
       TCAB_CASE(8, 1) TCAB_CASE(8, 2) TCAB_CASE(8, 4) TCAB_CASE(16, 4) TCAB_CASE(32, 4) TCAB_CASE(64, 4) TCAB_CASE(128, 4)
       TCAB_CASE(256, 4) TCAB_CASE(512, 4) TCAB_CASE(1024, 4) TCAB_CASE(128, 8) TCAB_CASE(256, 8) TCAB_CASE(512, 8)
       TCAB_CASE(64, 8) TCAB_CASE(1024, 8) TCAB_CASE(1024, 16)
@@ -720,13 +728,13 @@ int dispatch(const T* x, const T* gamma, const T* beta, float eps, T* y, uint64_
     const bool few_long = !many && nvec > 16384u;
     if (vec && tn.p0 <= 0 && rows * 8 <= 0x7fffffffull &&
         (tn.p3 == 7 || (tn.p3 <= 0 && ((pays && many) || few_long))))
-      return launch_cluster_stream<T, VW>(x, gamma, beta, eps, y, rows, cols, nvec, few_long, s);
+      return launch_cluster_stream<T, VW>(x, gamma, beta, eps, y, st, rows, cols, nvec, few_long, s);
   }
   const uint64_t row_bytes = static_cast<uint64_t>(cols) * sizeof(T);
   const bool smem_pays = sizeof(T) == 4 ? nvec >= 2560 : row_bytes > 32768;
   if (vec && tn.p0 <= 0 && rows_smem_fits(row_bytes) &&
       (tn.p3 == 4 || (tn.p3 <= 0 && smem_pays && rows >= static_cast<uint64_t>(sm_count()))))
-    return launch_smem(x, gamma, beta, eps, y, rows, cols, s);
+    return launch_smem(x, gamma, beta, eps, y, st, rows, cols, s);
   // Few long rows go to the cluster kernel (2-8 CTAs x 4096 vectors share a row, so a handful of rows
   // still spreads over the GPU: 64 x 131072 bf16 runs at 1.75 TB/s instead of 1.10). With many rows the
   // single-CTA kernels are faster (4.3 vs 2.6 TB/s at 4096 x 65536: three cluster barriers per row are
@@ -734,17 +742,17 @@ int dispatch(const T* x, const T* gamma, const T* beta, float eps, T* y, uint64_
   const bool few_rows = rows < 2ull * sm_count() && nvec > 8192;
   if (tn.p0 <= 0 && nvec > (tn.p3 == 3 ? 1024u : 4096u) && nvec <= 8u * 4096u && rows * 8 <= 0x7fffffffull && tn.p3 != 2 &&
       ((few_rows && nvec <= 16384) || tn.p3 == 3))
-    return vec ? launch_cluster<T, VW>(x, gamma, beta, eps, y, rows, cols, nvec, s)
-               : launch_cluster<T, 1>(x, gamma, beta, eps, y, rows, cols, nvec, s);
+    return vec ? launch_cluster<T, VW>(x, gamma, beta, eps, y, st, rows, cols, nvec, s)
+               : launch_cluster<T, 1>(x, gamma, beta, eps, y, st, rows, cols, nvec, s);
   if (fits) {
 #define TCAB_CASE(TP, P)                                                                         \
   if (tpr == TP && vpt == P)                                                                     \
-    return vec ? launch_reg<T, TP, P, VW>(x, gamma, beta, eps, y, rows, cols, tn.p2, s)          \
-               : launch_reg<T, TP, P, 1>(x, gamma, beta, eps, y, rows, cols, tn.p2, s);
+    return vec ? launch_reg<T, TP, P, VW>(x, gamma, beta, eps, y, st, rows, cols, tn.p2, s)          \
+               : launch_reg<T, TP, P, 1>(x, gamma, beta, eps, y, st, rows, cols, tn.p2, s);
     TCAB_LN_SHAPES_BASE(TCAB_CASE)
 #undef TCAB_CASE
 #define TCAB_CASE(TP, P) \
-  if (vec && tpr == TP && vpt == P) return launch_reg<T, TP, P, VW>(x, gamma, beta, eps, y, rows, cols, tn.p2, s);
+  if (vec && tpr == TP && vpt == P) return launch_reg<T, TP, P, VW>(x, gamma, beta, eps, y, st, rows, cols, tn.p2, s);
     TCAB_LN_SHAPES_EXTRA(TCAB_CASE)
 #undef TCAB_CASE
     if (tn.p0 > 0) return fail(TCAB_ERR_UNSUPPORTED, "layernorm: no kernel for tuned shape %d x %d", tpr, vpt);
@@ -753,9 +761,9 @@ int dispatch(const T* x, const T* gamma, const T* beta, float eps, T* y, uint64_
   const uint64_t cap = static_cast<uint64_t>(sm_count()) * 4;
   const unsigned grid = static_cast<unsigned>(rows < cap ? rows : cap);
   if (vec) {
-    layernorm_rows_stream<T, THREADS, VW><<<grid, THREADS, 0, s>>>(x, gamma, beta, eps, y, rows, cols);
+    layernorm_rows_stream<T, THREADS, VW><<<grid, THREADS, 0, s>>>(x, gamma, beta, eps, y, st, rows, cols);
   } else {
-    layernorm_rows_stream<T, THREADS, 1><<<grid, THREADS, 0, s>>>(x, gamma, beta, eps, y, rows, cols);
+    layernorm_rows_stream<T, THREADS, 1><<<grid, THREADS, 0, s>>>(x, gamma, beta, eps, y, st, rows, cols);
   }
   count_launch();
   return check_launch("layernorm_rows_stream");
@@ -764,14 +772,14 @@ int dispatch(const T* x, const T* gamma, const T* beta, float eps, T* y, uint64_
 }  // namespace
 
 int launch_layernorm_rows_bf16(const __nv_bfloat16* x, const __nv_bfloat16* gamma,
-                               const __nv_bfloat16* beta, float eps, __nv_bfloat16* y,
+                               const __nv_bfloat16* beta, float eps, __nv_bfloat16* y, RowStats st,
                                uint64_t rows, uint32_t cols, cudaStream_t s) {
-  return dispatch<__nv_bfloat16, 8>(x, gamma, beta, eps, y, rows, cols, s);
+  return dispatch<__nv_bfloat16, 8>(x, gamma, beta, eps, y, st, rows, cols, s);
 }
 
 int launch_layernorm_rows_f32(const float* x, const float* gamma, const float* beta, float eps,
-                              float* y, uint64_t rows, uint32_t cols, cudaStream_t s) {
-  return dispatch<float, 4>(x, gamma, beta, eps, y, rows, cols, s);
+                              float* y, RowStats st, uint64_t rows, uint32_t cols, cudaStream_t s) {
+  return dispatch<float, 4>(x, gamma, beta, eps, y, st, rows, cols, s);
 }
 
 }  // namespace tcab

@@ -145,7 +145,7 @@ __device__ __forceinline__ void finish_ring(Ring<CF>& ring) {
 template <class CF, typename T, int V, bool SHIFTED, bool PF = false>
 __global__ void __launch_bounds__(CF::kThreads, PF ? 12 / CF::kSlots : 1)
 layernorm_rows_smem(const T* __restrict__ x, const T* __restrict__ gamma, const T* __restrict__ beta, float eps,
-                    T* __restrict__ y, uint64_t rows, uint32_t cols) {
+                    T* __restrict__ y, RowStats st, uint64_t rows, uint32_t cols) {
   using IO = VecIO<T, V>;
   using Raw = typename IO::Raw;
   constexpr int kSlots = CF::kSlots, kConsumers = CF::kConsumers;
@@ -296,6 +296,7 @@ layernorm_rows_smem(const T* __restrict__ x, const T* __restrict__ gamma, const 
       }
       rstd = 1.0f / sqrtf(consumers_allreduce<CF, OpSum>(q, red_b) / n + eps);
       }
+      if (threadIdx.x == 0) st.put(row, mean, rstd);
       // pass 3: normalise, scale, shift, store; hand each slot back once this warp has read it
       {
         uint32_t slot = slot0;
@@ -498,31 +499,31 @@ int launch_softmax_rows_smem(const float* x, float* y, uint64_t rows, uint32_t c
 }
 
 int launch_layernorm_rows_smem_bf16(const __nv_bfloat16* x, const __nv_bfloat16* gamma, const __nv_bfloat16* beta,
-                                    float eps, __nv_bfloat16* y, uint64_t rows, uint32_t cols, cudaStream_t s) {
+                                    float eps, __nv_bfloat16* y, RowStats st, uint64_t rows, uint32_t cols, cudaStream_t s) {
   typedef __nv_bfloat16 B;
   const bool pf = tune(kLayernorm).p1 != 8;  // p1 == 8: no gamma / beta prefetch (for comparisons)
   switch (pick_cfg(static_cast<uint64_t>(cols) * 2, tune(kLayernorm).p2)) {
-    case 2: return launch_cfg<Third>(layernorm_rows_smem<Third, B, 8, true>, 3, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, rows, cols);
+    case 2: return launch_cfg<Third>(layernorm_rows_smem<Third, B, 8, true>, 3, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, st, rows, cols);
     case 1:
-      if (pf) return launch_cfg<Half>(layernorm_rows_smem<Half, B, 8, true, true>, 2, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, rows, cols);
-      return launch_cfg<Half>(layernorm_rows_smem<Half, B, 8, true>, 2, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, rows, cols);
+      if (pf) return launch_cfg<Half>(layernorm_rows_smem<Half, B, 8, true, true>, 2, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, st, rows, cols);
+      return launch_cfg<Half>(layernorm_rows_smem<Half, B, 8, true>, 2, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, st, rows, cols);
     default:
-      if (pf) return launch_cfg<Whole>(layernorm_rows_smem<Whole, B, 8, true, true>, 1, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, rows, cols);
-      return launch_cfg<Whole>(layernorm_rows_smem<Whole, B, 8, true>, 1, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, rows, cols);
+      if (pf) return launch_cfg<Whole>(layernorm_rows_smem<Whole, B, 8, true, true>, 1, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, st, rows, cols);
+      return launch_cfg<Whole>(layernorm_rows_smem<Whole, B, 8, true>, 1, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, st, rows, cols);
   }
 }
 
-int launch_layernorm_rows_smem_f32(const float* x, const float* gamma, const float* beta, float eps, float* y,
+int launch_layernorm_rows_smem_f32(const float* x, const float* gamma, const float* beta, float eps, float* y, RowStats st,
                                    uint64_t rows, uint32_t cols, cudaStream_t s) {
   const bool pf = tune(kLayernorm).p1 != 8;
   switch (pick_cfg(static_cast<uint64_t>(cols) * 4, tune(kLayernorm).p2)) {
-    case 2: return launch_cfg<Third>(layernorm_rows_smem<Third, float, 4, false>, 3, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, rows, cols);
+    case 2: return launch_cfg<Third>(layernorm_rows_smem<Third, float, 4, false>, 3, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, st, rows, cols);
     case 1:
-      if (pf) return launch_cfg<Half>(layernorm_rows_smem<Half, float, 4, false, true>, 2, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, rows, cols);
-      return launch_cfg<Half>(layernorm_rows_smem<Half, float, 4, false>, 2, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, rows, cols);
+      if (pf) return launch_cfg<Half>(layernorm_rows_smem<Half, float, 4, false, true>, 2, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, st, rows, cols);
+      return launch_cfg<Half>(layernorm_rows_smem<Half, float, 4, false>, 2, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, st, rows, cols);
     default:
-      if (pf) return launch_cfg<Whole>(layernorm_rows_smem<Whole, float, 4, false, true>, 1, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, rows, cols);
-      return launch_cfg<Whole>(layernorm_rows_smem<Whole, float, 4, false>, 1, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, rows, cols);
+      if (pf) return launch_cfg<Whole>(layernorm_rows_smem<Whole, float, 4, false, true>, 1, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, st, rows, cols);
+      return launch_cfg<Whole>(layernorm_rows_smem<Whole, float, 4, false>, 1, rows, s, "layernorm_rows_smem", x, gamma, beta, eps, y, st, rows, cols);
   }
 }
 

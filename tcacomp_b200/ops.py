@@ -398,3 +398,185 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
                                                   C.byref(biasv) if biasv is not None else None, code,
                                                   C.byref(cv), _stream(stream, a)))
     return out
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# a feed-forward sublayer and its training step
+# ---------------------------------------------------------------------------------------------------------------------
+_ACTS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU,
+         "gelu_tanh": _lib.ACT_GELU_TANH, "sigmoid": _lib.ACT_SIGMOID}
+_PLAIN_ACTS = ("none", "relu", "silu", "gelu", "gelu_tanh")
+_GATE_ACTS = ("silu", "gelu", "gelu_tanh", "sigmoid", "relu")
+
+
+def _act_code(act: str, allowed: Sequence[str]) -> int:
+    if act not in allowed:
+        raise ValueError(f"unknown activation {act!r} (one of {', '.join(allowed)})")
+    return _ACTS[act]
+
+
+def _allocating(stream: Optional[torch.cuda.Stream]):
+    """Tensors made inside belong to the stream the call runs on: memory that another stream may still be using is not
+    handed out for them, and a workspace that is dropped on return is not handed on before the call's work is done."""
+    return _ALREADY_CURRENT if stream is None else torch.cuda.stream(stream)
+
+
+def _ref(t: Optional[torch.Tensor], name: str):
+    return None if t is None else C.byref(_view(t, name))
+
+
+def _workspace(nbytes: int, ref: torch.Tensor) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, device=ref.device, dtype=torch.uint8) if nbytes else None
+
+
+def _ptr(ws: Optional[torch.Tensor]):
+    return C.c_void_p(ws.data_ptr() if ws is not None else 0)
+
+
+def layernorm_rows_stats(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps: float = 1e-5,
+                         out: Optional[torch.Tensor] = None, mean: Optional[torch.Tensor] = None,
+                         rstd: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> tuple:
+    """layernorm_rows that also returns what its backward pass needs: (y, mean, rstd), the statistics fp32 with the
+    extents of x without the innermost one (rank-1 x: [1])."""
+    xv = _view(x, "x")
+    with _on_device(x):
+        if out is None or mean is None or rstd is None:
+            with _allocating(stream):
+                shape = x.shape[:-1] or (1,)
+                out = torch.empty_like(x) if out is None else out
+                mean = torch.empty(shape, device=x.device, dtype=torch.float32) if mean is None else mean
+                rstd = torch.empty(shape, device=x.device, dtype=torch.float32) if rstd is None else rstd
+        gv, bv, yv, mv, rv = _view(gamma, "gamma"), _view(beta, "beta"), _view(out, "out"), _view(mean, "mean"), _view(rstd, "rstd")
+        _same_device(("x", x), ("gamma", gamma), ("beta", beta), ("out", out), ("mean", mean), ("rstd", rstd))
+        _lib.check(_lib.load().tcab_layernorm_rows_stats(C.byref(xv), C.byref(gv), C.byref(bv), C.c_float(eps), C.byref(yv),
+                                                         C.byref(mv), C.byref(rv), _stream(stream, x)))
+    return out, mean, rstd
+
+
+def layernorm_rows_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                            dx: Optional[torch.Tensor] = None, dgamma: Optional[torch.Tensor] = None,
+                            dbeta: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> tuple:
+    """Backward pass of layernorm_rows_stats: (dx, dgamma, dbeta). dx has the type of x (it may be dy or x themselves),
+    dgamma and dbeta are fp32."""
+    xv = _view(x, "x")
+    lib = _lib.load()
+    with _on_device(x):
+        with _allocating(stream):
+            cols = x.shape[-1]
+            dx = torch.empty_like(x) if dx is None else dx
+            dgamma = torch.empty(cols, device=x.device, dtype=torch.float32) if dgamma is None else dgamma
+            dbeta = torch.empty(cols, device=x.device, dtype=torch.float32) if dbeta is None else dbeta
+            nbytes = lib.tcab_layernorm_rows_backward_workspace(C.byref(xv))
+            ws = _workspace(nbytes, x)
+        _same_device(("x", x), ("dy", dy), ("gamma", gamma), ("mean", mean), ("rstd", rstd), ("dx", dx), ("dgamma", dgamma),
+                     ("dbeta", dbeta))
+        _lib.check(lib.tcab_layernorm_rows_backward(
+            _ref(dy, "dy"), C.byref(xv), _ref(gamma, "gamma"), _ref(mean, "mean"), _ref(rstd, "rstd"), _ref(dx, "dx"),
+            _ref(dgamma, "dgamma"), _ref(dbeta, "dbeta"), _ptr(ws), nbytes, _stream(stream, x)))
+    return dx, dgamma, dbeta
+
+
+def gemm_bias_act_residual(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                           residual: Optional[torch.Tensor] = None, act: str = "gelu", out: Optional[torch.Tensor] = None,
+                           preact: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """c = act(a @ b + bias) + residual: a [M,K] bf16, b [K,N] bf16, bias [N] fp32, residual and c [M,N] bf16; act one of
+    none, relu, silu, gelu, gelu_tanh. preact [M,N] bf16, where given, receives a @ b + bias for the backward pass. c may
+    be the residual itself (out=residual)."""
+    code = _act_code(act, _PLAIN_ACTS)
+    av, bv = _view(a, "a"), _view(b, "b")
+    if av.rank != 2 or bv.rank != 2:
+        raise ValueError("a and b must be rank 2")
+    with _on_device(a):
+        if out is None:
+            with _allocating(stream):
+                out = torch.empty((a.shape[0], b.shape[1]), device=a.device, dtype=torch.bfloat16)
+        _same_device(("a", a), ("b", b), ("bias", bias), ("residual", residual), ("out", out), ("preact", preact))
+        _lib.check(_lib.load().tcab_gemm_bias_act_residual(
+            C.byref(av), C.byref(bv), _ref(bias, "bias"), _ref(residual, "residual"), code, _ref(preact, "preact"),
+            _ref(out, "out"), _stream(stream, a)))
+    return out
+
+
+def _wanted(want: Sequence[str], known: Sequence[str], out: Optional[dict], shapes: dict, ref: torch.Tensor) -> dict:
+    """The outputs a backward pass is to compute, by name: the caller's where given, new ones otherwise."""
+    res = dict(out or {})
+    for name in list(res) + list(want):
+        if name not in known:
+            raise ValueError(f"unknown output {name!r} (one of {', '.join(known)})")
+    for name in want:
+        if name not in res:
+            res[name] = torch.empty(shapes[name], device=ref.device,
+                                    dtype=torch.float32 if name.startswith("dbias") else torch.bfloat16)
+    return res
+
+
+def gemm_bias_act_backward(dc: torch.Tensor, a: torch.Tensor, b: torch.Tensor, preact: Optional[torch.Tensor] = None,
+                           act: str = "gelu", want: Sequence[str] = ("da", "db", "dbias"), out: Optional[dict] = None,
+                           stream: Optional[torch.cuda.Stream] = None) -> dict:
+    """Backward pass of gemm_bias_act_residual; returns {"da" [M,K] bf16, "db" [K,N] bf16, "dbias" [N] fp32} as requested
+    (the gradient of the residual is dc). preact is what the forward pass stored; it is not needed for act="none"."""
+    code = _act_code(act, _PLAIN_ACTS)
+    av, bv = _view(a, "a"), _view(b, "b")
+    if av.rank != 2 or bv.rank != 2:
+        raise ValueError("a and b must be rank 2")
+    m, k, n = a.shape[0], a.shape[1], b.shape[1]
+    lib = _lib.load()
+    with _on_device(a):
+        with _allocating(stream):
+            res = _wanted(want, ("da", "db", "dbias"), out, {"da": (m, k), "db": (k, n), "dbias": (n,)}, a)
+            nbytes = lib.tcab_gemm_bias_act_backward_workspace(m, n, code, int("dbias" in res))
+            ws = _workspace(nbytes, a)
+        _same_device(("a", a), ("b", b), ("dc", dc), ("preact", preact), *res.items())
+        _lib.check(lib.tcab_gemm_bias_act_backward(
+            _ref(dc, "dc"), C.byref(av), C.byref(bv), _ref(preact, "preact"), code, _ref(res.get("da"), "da"),
+            _ref(res.get("db"), "db"), _ref(res.get("dbias"), "dbias"), _ptr(ws), nbytes, _stream(stream, a)))
+    return res
+
+
+def gated_gemm(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, bias_gate: Optional[torch.Tensor] = None,
+               bias_up: Optional[torch.Tensor] = None, act: str = "silu", out: Optional[torch.Tensor] = None,
+               gate: Optional[torch.Tensor] = None, up: Optional[torch.Tensor] = None,
+               stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """h = act(x @ w_gate + bias_gate) * (x @ w_up + bias_up) in one kernel: x [M,K], w_gate and w_up [K,N], h [M,N] bf16,
+    the biases [N] fp32 (both or neither); act one of silu, gelu, gelu_tanh, sigmoid, relu. gate and up [M,N] bf16 (both or
+    neither) receive the two projections for the backward pass."""
+    code = _act_code(act, _GATE_ACTS)
+    xv, gv = _view(x, "x"), _view(w_gate, "w_gate")
+    if xv.rank != 2 or gv.rank != 2:
+        raise ValueError("x and w_gate must be rank 2")
+    with _on_device(x):
+        if out is None:
+            with _allocating(stream):
+                out = torch.empty((x.shape[0], w_gate.shape[1]), device=x.device, dtype=torch.bfloat16)
+        _same_device(("x", x), ("w_gate", w_gate), ("w_up", w_up), ("bias_gate", bias_gate), ("bias_up", bias_up), ("out", out),
+                     ("gate", gate), ("up", up))
+        _lib.check(_lib.load().tcab_gated_gemm(
+            C.byref(xv), C.byref(gv), _ref(w_up, "w_up"), _ref(bias_gate, "bias_gate"), _ref(bias_up, "bias_up"), code,
+            _ref(gate, "gate"), _ref(up, "up"), _ref(out, "out"), _stream(stream, x)))
+    return out
+
+
+def gated_gemm_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, gate: torch.Tensor,
+                        up: torch.Tensor, act: str = "silu", want: Sequence[str] = ("dx", "dw_gate", "dw_up"),
+                        out: Optional[dict] = None, stream: Optional[torch.cuda.Stream] = None) -> dict:
+    """Backward pass of gated_gemm from the projections it stored; returns {"dx" [M,K], "dw_gate" and "dw_up" [K,N] bf16,
+    "dbias_gate" and "dbias_up" [N] fp32} as requested (the weights' gradients both or neither, the biases' likewise)."""
+    code = _act_code(act, _GATE_ACTS)
+    xv, gv = _view(x, "x"), _view(w_gate, "w_gate")
+    if xv.rank != 2 or gv.rank != 2:
+        raise ValueError("x and w_gate must be rank 2")
+    m, k, n = x.shape[0], x.shape[1], w_gate.shape[1]
+    known = {"dx": (m, k), "dw_gate": (k, n), "dw_up": (k, n), "dbias_gate": (n,), "dbias_up": (n,)}
+    lib = _lib.load()
+    with _on_device(x):
+        with _allocating(stream):
+            res = _wanted(want, tuple(known), out, known, x)
+            nbytes = lib.tcab_gated_gemm_backward_workspace(m, n, int("dbias_gate" in res or "dbias_up" in res))
+            ws = _workspace(nbytes, x)
+        _same_device(("x", x), ("w_gate", w_gate), ("w_up", w_up), ("dh", dh), ("gate", gate), ("up", up), *res.items())
+        _lib.check(lib.tcab_gated_gemm_backward(
+            _ref(dh, "dh"), C.byref(xv), C.byref(gv), _ref(w_up, "w_up"), _ref(gate, "gate"), _ref(up, "up"), code,
+            _ref(res.get("dx"), "dx"), _ref(res.get("dw_gate"), "dw_gate"), _ref(res.get("dw_up"), "dw_up"),
+            _ref(res.get("dbias_gate"), "dbias_gate"), _ref(res.get("dbias_up"), "dbias_up"), _ptr(ws), nbytes,
+            _stream(stream, x)))
+    return res
