@@ -146,6 +146,22 @@ def load() -> C.CDLL:
     return lib
 
 
+_PACKED: dict = {}
+
+
+def packed(name: str):
+    """The function `name` taking its tensors as bytes objects that hold a tcab_tensor (or None), for operators of many
+    tensors: a prototype of its own beside the one load() binds."""
+    fn = _PACKED.get(name)
+    if fn is None:
+        restype, argtypes = next((r, a) for n, r, a in SYMBOLS if n == name)
+        fn = load()[name]  # a new function object: load()'s keeps its own argument types
+        fn.restype = restype
+        fn.argtypes = [C.c_char_p if a is C.POINTER(Tensor) else a for a in argtypes]
+        _PACKED[name] = fn
+    return fn
+
+
 def check(status: int) -> None:
     if status != OK:
         raise TcabError(status, load().tcab_last_error().decode("utf-8", "replace"))

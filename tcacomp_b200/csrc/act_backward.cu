@@ -58,23 +58,22 @@ act_backward_kernel(const __nv_bfloat16* __restrict__ in0, const __nv_bfloat16* 
       const uint64_t row = row0 + u * step;
       if (row >= rows) continue;
       const uint64_t at = row * nvec + v;
-      float d[8], z[8], up[8], o1[8];
+      float d[8], up[8], o1[8];
       IO::unpack(q0[u], d);
-      if (ACT != TCAB_ACT_NONE) IO::unpack(q1[u], z);
-      if (GATED) IO::unpack(q2[u], up);
+      if constexpr (ACT != TCAB_ACT_NONE) {
+        float z[8], value[8], slope[8];
+        IO::unpack(q1[u], z);
+        if (GATED) IO::unpack(q2[u], up);
+        act_values_slopes<ACT>(z, value, slope);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (ACT != TCAB_ACT_NONE) {
-          float value, slope;
-          act_value_slope<ACT>(z[j], &value, &slope);
-          if (GATED) {
-            o1[j] = d[j] * value;
-            d[j] = d[j] * up[j] * slope;
-          } else {
-            d[j] *= slope;
-          }
+        for (int j = 0; j < 8; ++j) {
+          if (GATED) o1[j] = d[j] * value[j];
+          d[j] = (GATED ? d[j] * up[j] : d[j]) * slope[j];
         }
-        if (SUMS) {
+      }
+      if constexpr (SUMS) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
           acc[0][j] += d[j];
           if (GATED) acc[NS - 1][j] += o1[j];
         }

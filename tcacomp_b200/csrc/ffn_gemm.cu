@@ -41,19 +41,20 @@ FfnKernel kernel_of(int form, int act, int shape) {
   }
 }
 
-constexpr int kBM[3] = {256, 128, 128}, kBN[3] = {256, 256, 128};
+// The tile shapes of ffn_kernel_of.
+constexpr int kShapes = 3, kCtas[kShapes] = {2, 2, 1}, kRows[kShapes] = {512, 256, 128}, kBN[kShapes] = {256, 256, 128};
 
-// The tile shape: fewest rounds over the SMs, weighted by what a tile of each shape costs (a 128-row tile moves more
-// bytes per product through shared memory and ran at about 0.8 of the 256 x 256 tile's rate, 128 x 128 at 0.6).
+// The tile shape: fewest rounds over the SMs (pairs of SMs), weighted by what a round of each shape costs.
 int pick_shape(int form, const FfnProblem& p) {
-  static const double kCost[3] = {1.0, 0.5 / 0.8, 0.25 / 0.6};
+  static const double kCost[kShapes] = {1.0, 0.55, 0.36};  // of a round of one tile per CTA or pair
   const uint64_t sms = static_cast<uint64_t>(sm_count()), outs = form == kFfnDw && p.b[1] != nullptr ? 2 : 1;
   int best = 0;
   double best_cost = 1e300;
-  for (int s = 0; s < 3; ++s) {
-    const uint64_t tn = static_cast<uint64_t>(form == kFfnGated ? kBN[s] / 2 : kBN[s]);
-    const uint64_t tiles = (p.M + kBM[s] - 1) / kBM[s] * ((p.N + tn - 1) / tn) * outs;
-    const double cost = static_cast<double>((tiles + sms - 1) / sms) * kCost[s];
+  for (int s = 0; s < kShapes; ++s) {
+    const uint64_t bm = kRows[s], tn = static_cast<uint64_t>(form == kFfnGated ? kBN[s] / 2 : kBN[s]);
+    const uint64_t tiles = (p.M + bm - 1) / bm * ((p.N + tn - 1) / tn) * outs, at_once = sms / kCtas[s];
+    if (at_once == 0) continue;
+    const double cost = static_cast<double>((tiles + at_once - 1) / at_once) * kCost[s];
     if (cost < best_cost - 1e-9) {
       best_cost = cost;
       best = s;
@@ -84,8 +85,8 @@ int ffn_device_status(int* out) {
 int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t s) {
   if (p.M == 0 || p.N == 0) return TCAB_OK;
   const Tune& tn = tune(kFfn);
-  const int shape = tn.p1 > 0 && tn.p1 <= 3 ? tn.p1 - 1 : pick_shape(form, p);
-  const uint32_t bm = kBM[shape], bn = kBN[shape], tile_n = form == kFfnGated ? bn / 2 : bn;
+  const int shape = tn.p1 > 0 && tn.p1 <= kShapes ? tn.p1 - 1 : pick_shape(form, p);
+  const uint32_t ctas = kCtas[shape], bm = kRows[shape], bn = kBN[shape], tile_n = form == kFfnGated ? bn / 2 : bn;
   FfnArgs args = {};
   args.M = p.M;
   args.N = p.N;
@@ -100,11 +101,11 @@ int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t 
     if (form == kFfnDw) {
       TCAB_TRY_RC(make_tensor_map(op, &args.a[0], p.a[0], p.K, p.M, 64, 64));
     } else {
-      TCAB_TRY_RC(make_tensor_map(op, &args.a[0], p.a[0], p.M, p.K, bm, 64));
-      if (form == kFfnDx && nb == 2) TCAB_TRY_RC(make_tensor_map(op, &args.a[1], p.a[1], p.M, p.K, bm, 64));
+      TCAB_TRY_RC(make_tensor_map(op, &args.a[0], p.a[0], p.M, p.K, 128, 64));
+      if (form == kFfnDx && nb == 2) TCAB_TRY_RC(make_tensor_map(op, &args.a[1], p.a[1], p.M, p.K, 128, 64));
     }
     for (int i = 0; i < nb; ++i) {
-      if (form == kFfnDx) TCAB_TRY_RC(make_tensor_map(op, &args.b[i], p.b[i], p.N, p.K, bn, 64));
+      if (form == kFfnDx) TCAB_TRY_RC(make_tensor_map(op, &args.b[i], p.b[i], p.N, p.K, bn / ctas, 64));
       else TCAB_TRY_RC(make_tensor_map(op, &args.b[i], p.b[i], p.K, p.N, 64, 64));
     }
   }
@@ -121,10 +122,23 @@ int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t 
     return fail(TCAB_ERR_CUDA, "%s: cannot reserve %zu bytes of shared memory: %s", op, k.smem, cudaGetErrorString(ae));
   }
   const uint64_t tiles = static_cast<uint64_t>((p.M + bm - 1) / bm) * ((p.N + tile_n - 1) / tile_n) * (form == kFfnDw ? nb : 1);
-  uint64_t grid = tn.p0 > 0 ? static_cast<uint64_t>(tn.p0) : static_cast<uint64_t>(sm_count());
-  if (grid > tiles) grid = tiles;
+  uint64_t groups = (tn.p0 > 0 ? static_cast<uint64_t>(tn.p0) : static_cast<uint64_t>(sm_count())) / ctas;
+  if (groups > tiles) groups = tiles;
+  if (groups < 1) groups = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(groups * ctas));
+  cfg.blockDim = dim3(kFfnThreads);
+  cfg.dynamicSmemBytes = k.smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   void* params[] = {&args};
-  const cudaError_t le = cudaLaunchKernel(k.fn, dim3(static_cast<unsigned>(grid)), dim3(kFfnThreads), params, k.smem, s);
+  const cudaError_t le = cudaLaunchKernelExC(&cfg, k.fn, params);
   count_launch();
   if (le != cudaSuccess) {
     cudaGetLastError();

@@ -9,12 +9,11 @@
 //   Dx      [M, K] (twice)         [N, K] (twice), K-major                 BN rows; the K loop runs over both pairs
 //   Dw      [K, M], M-major        [K, N] (twice), N-major                 BN columns; tiles of the second output follow
 //
-// Roles: warp 0 (one lane) is the TMA producer, warp 1 (one lane) issues the MMAs, warps 2-9 are the epilogue. A K block
-// is 64 wide; a tile of BM x BN takes BM / 128 accumulators of 128 x BN, and TMEM holds 512 / BN of them in a ring, so
-// that with BM = 128 the epilogue of a tile runs under the K loop of the next. With BM = BN = 256 the two accumulators
-// of a tile fill TMEM: a warp pulls its whole share of the first into registers, hands it back, and refills each
-// register block from the second as soon as it has been consumed (what costs time there is how long the next tile's
-// first MMAs wait for an accumulator, see gemm_bias_act.cu).
+// A tile is 256 x 256 on a pair of CTAs (cta_group::2: each loads its 128 rows of a and half of b's columns, the
+// leader issues the MMAs), or 128 x 256 or 128 x 128 on one CTA. Roles: warp 0 (one lane) is the TMA producer, warp 1
+// (one lane) issues the MMAs, warps 4-11 are the epilogue (and take most of the registers). A K block is 64 wide; a CTA's accumulator is 128 x BN, and TMEM
+// holds 512 / BN of them in a ring, so that the epilogue of a tile -- activations, products, residuals, up to three stored
+// matrices -- runs under the K loop of the next. It takes 32 columns at a time, with the next 32 under way from TMEM.
 //
 // Results leave through 32 x 32 boxes in two alternating staging buffers per warp and TMA stores, which clip ragged
 // edges. Loads past an edge read zeros. Every wait is bounded (sm100_ptx.cuh); a wait that gives up ends the kernel
@@ -27,7 +26,7 @@
 
 namespace tcab {
 
-constexpr int kFfnBK = 64, kFfnEpiWarps = 8, kFfnThreads = 64 + 32 * kFfnEpiWarps;
+constexpr int kFfnBK = 64, kFfnEpiWarps = 8, kFfnThreads = 128 + 32 * kFfnEpiWarps;
 constexpr int kFfnAtom = kFfnBK * 128;  // a box of 64 x 64 bf16
 constexpr int kFfnStageBox = 32 * 64;   // a box of 32 x 32 bf16 results
 
@@ -48,11 +47,13 @@ struct FfnKernel {
   cudaError_t (*status)(int*);
 };
 
-template <int BM, int BN>
+// A tile of (128 NACC CTAS) x BN on CTAS SMs. A CTA holds NACC accumulators of 128 rows x BN columns of it and loads, per
+// K block, the 128 NACC rows of a that belong to them and BN / CTAS columns of b. KPS K blocks share a ring stage.
+template <int CTAS, int NACC_, int BN, int KPS_>
 struct FfnTile {
-  static constexpr int NACC = BM / 128, SLOTS = 512 / BN;
-  static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = (BM + BN >= 512) ? 3 : (BM + BN >= 384) ? 4 : 6;
+  static constexpr int NACC = NACC_, KPS = KPS_, BM = 128 * NACC * CTAS, B_COLS = BN / CTAS, SLOTS = 512 / BN;
+  static constexpr int A_BYTES = NACC * 128 * 128, B_BYTES = B_COLS * 128, BLOCK = A_BYTES + B_BYTES, STAGE = KPS * BLOCK;
+  static constexpr int STAGES = 192 * 1024 / STAGE;
   static constexpr size_t SMEM = static_cast<size_t>(STAGES) * STAGE + kFfnEpiWarps * 2 * kFfnStageBox + 1024;
 };
 
@@ -71,32 +72,36 @@ __device__ int g_ffn_status = 0;
 
 cudaError_t read_status(int* out) { return cudaMemcpyFromSymbol(out, g_ffn_status, sizeof(int)); }
 
-template <int FORM, int ACT, int BM, int BN>
+template <int FORM, int ACT, int CTAS, int NACC, int BN, int KPS>
 __global__ void __launch_bounds__(kFfnThreads, 1)
 ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
-  using C = FfnTile<BM, BN>;
+  using C = FfnTile<CTAS, NACC, BN, KPS>;
+  constexpr bool PAIR = CTAS == 2;
   constexpr bool A_MN = FORM == kFfnDw, B_NK = FORM == kFfnDx, GATED = FORM == kFfnGated;
   constexpr bool EPILOGUE = FORM == kFfnFwd || FORM == kFfnGated;
   constexpr int TN = GATED ? BN / 2 : BN;  // output columns per tile
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_full[C::STAGES];
-  __shared__ __align__(8) uint64_t bar_empty[C::STAGES];
-  __shared__ __align__(8) uint64_t bar_acc_full[C::SLOTS];
-  __shared__ __align__(8) uint64_t bar_acc_empty[C::SLOTS];
+  __shared__ __align__(8) uint64_t bar_full[C::STAGES];       // PAIR: used in the leader, bytes of both CTAs land here
+  __shared__ __align__(8) uint64_t bar_empty[C::STAGES];      // in each CTA
+  __shared__ __align__(8) uint64_t bar_acc_full[C::SLOTS];    // in each CTA
+  __shared__ __align__(8) uint64_t bar_acc_empty[C::SLOTS];   // PAIR: used in the leader, both CTAs' epilogue warps arrive
   __shared__ __align__(16) float bias_s[EPILOGUE ? BN : 4];  // the current tile's (zeros past N)
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
 
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? ptx::cluster_ctarank() : 0u;
+  const bool leader = rank == 0;
   volatile int* abort_p = &abort_flag;
 
   const uint32_t M = args.M, N = args.N;
-  const uint32_t tiles_m = (M + BM - 1) / BM, tiles_n1 = (N + TN - 1) / TN;
+  const uint32_t tiles_m = (M + C::BM - 1) / C::BM, tiles_n1 = (N + TN - 1) / TN;
   const uint32_t tiles_one = tiles_m * tiles_n1;  // tiles of one output
   const uint32_t num_tiles = FORM == kFfnDw ? tiles_one * args.pairs : tiles_one;
-  const uint32_t seg_kb = (args.K + kFfnBK - 1) / kFfnBK;
-  const uint32_t num_kb = FORM == kFfnDx ? seg_kb * args.pairs : seg_kb;
+  const uint32_t seg_st = (args.K + kFfnBK * KPS - 1) / (kFfnBK * KPS);  // ring stages per contracted pair
+  const uint32_t num_st = FORM == kFfnDx ? seg_st * args.pairs : seg_st;
+  const uint32_t first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -106,95 +111,158 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
     }
     for (int s = 0; s < C::SLOTS; ++s) {
       ptx::mbar_init(ptx::smem_u32(&bar_acc_full[s]), 1);
-      ptx::mbar_init(ptx::smem_u32(&bar_acc_empty[s]), kFfnEpiWarps);
+      ptx::mbar_init(ptx::smem_u32(&bar_acc_empty[s]), CTAS * kFfnEpiWarps);
     }
     ptx::fence_barrier_init();
     ptx::fence_proxy_async();
   }
   if (warp == 1) {
-    ptx::tmem_alloc(ptx::smem_u32(&tmem_base_slot), 512);
-    ptx::tmem_relinquish();
+    if (PAIR) {
+      ptx::tmem_alloc_pair(ptx::smem_u32(&tmem_base_slot), 512);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(ptx::smem_u32(&tmem_base_slot), 512);
+      ptx::tmem_relinquish();
+    }
   }
   ptx::tc_fence_before();
   __syncthreads();
+  if (PAIR) {  // the peer's barriers must be initialised before anything of this CTA can signal them
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+  }
   ptx::tc_fence_after();
   const uint32_t tmem_base = tmem_base_slot;
 
-  if (warp == 0) {
-    // ---------------- TMA producer ----------------
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0;
-      bool ok = true;
-      for (uint32_t t = blockIdx.x; ok && t < num_tiles; t += gridDim.x) {
-        const uint32_t which = FORM == kFfnDw && t >= tiles_one ? 1u : 0u;
-        const FfnCoord tc = ffn_coord(t - which * tiles_one, tiles_m, tiles_n1);
-        const int32_t m0 = static_cast<int32_t>(tc.m * BM), n0 = static_cast<int32_t>(tc.n * TN);
-        for (uint32_t kb = 0; kb < num_kb; ++kb) {
-          if (!ptx::mbar_wait(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, abort_p)) { ok = false; break; }
-          const uint32_t full = ptx::smem_u32(&bar_full[stage]);
-          const uint32_t a_dst = smem_base + stage * C::STAGE, b_dst = a_dst + C::A_BYTES;
-          const uint32_t seg = FORM == kFfnDx && kb >= seg_kb ? 1u : 0u;
-          const int32_t k0 = static_cast<int32_t>((kb - seg * seg_kb) * kFfnBK);
-          ptx::mbar_expect_tx(full, C::STAGE);
-          if (A_MN) {
+  // Register split: 384 threads x 168 at launch = 64,512; 128 x 40 + 256 x 224 = 62,464 afterwards.
+  if (warp < 4) {
+    ptx::setmaxnreg_dec<40>();
+    if (warp == 0) {
+      // ---------------- TMA producer (every CTA) ----------------
+      if (lane == 0) {
+        auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y) {
+          if (PAIR) ptx::tma_load_2d_pair(dst, map, bar, x, y);
+          else ptx::tma_load_2d(dst, map, bar, x, y);
+        };
+        uint32_t stage = 0, phase = 0;
+        bool ok = true;
+        for (uint32_t t = first; ok && t < num_tiles; t += step) {
+          const uint32_t which = FORM == kFfnDw && t >= tiles_one ? 1u : 0u;
+          const FfnCoord tc = ffn_coord(t - which * tiles_one, tiles_m, tiles_n1);
+          const int32_t m0 = static_cast<int32_t>(tc.m * C::BM + rank * 128);  // accumulator a: + a * 128 CTAS
+          // Gated: a pair's first CTA loads the gate's columns, its second the same columns of up
+          const int32_t n0 = static_cast<int32_t>(tc.n * TN + (GATED ? 0u : rank * C::B_COLS));
+          for (uint32_t st = 0; st < num_st; ++st) {
+            if (!ptx::mbar_wait_parked(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, abort_p)) { ok = false; break; }
+            const uint32_t full = PAIR ? ptx::mapa(ptx::smem_u32(&bar_full[stage]), 0) : ptx::smem_u32(&bar_full[stage]);
+            const uint32_t seg = FORM == kFfnDx && st >= seg_st ? 1u : 0u;
+            if (leader) ptx::mbar_expect_tx(ptx::smem_u32(&bar_full[stage]), CTAS * C::STAGE);
 #pragma unroll
-            for (int j = 0; j < BM / 64; ++j) ptx::tma_load_2d(a_dst + j * kFfnAtom, &args.a[0], full, m0 + j * 64, k0);
-          } else {
-            ptx::tma_load_2d(a_dst, &args.a[seg], full, k0, m0);
+            for (int kk = 0; kk < KPS; ++kk) {
+              const uint32_t a_dst = smem_base + stage * C::STAGE + kk * C::BLOCK, b_dst = a_dst + C::A_BYTES;
+              const int32_t k0 = static_cast<int32_t>(((st - seg * seg_st) * KPS + kk) * kFfnBK);
+#pragma unroll
+              for (int a = 0; a < NACC; ++a) {
+                const int32_t row = m0 + a * 128 * CTAS;
+                if (A_MN) {
+                  load(a_dst + a * 2 * kFfnAtom, &args.a[0], full, row, k0);
+                  load(a_dst + a * 2 * kFfnAtom + kFfnAtom, &args.a[0], full, row + 64, k0);
+                } else {
+                  load(a_dst + a * 2 * kFfnAtom, &args.a[seg], full, k0, row);
+                }
+              }
+              if (B_NK) {
+                load(b_dst, &args.b[seg], full, k0, n0);
+              } else {
+#pragma unroll
+                for (int j = 0; j < C::B_COLS / 64; ++j) {
+                  constexpr int per = GATED && !PAIR ? BN / 128 : 64;  // Gated on one CTA: boxes of gate, then of up
+                  const uint32_t side = GATED ? (PAIR ? rank : static_cast<uint32_t>(j / per)) : which;
+                  load(b_dst + j * kFfnAtom, &args.b[side], full, n0 + (j % per) * 64, k0);
+                }
+              }
+            }
+            if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
           }
-          if (B_NK) {
-            ptx::tma_load_2d(b_dst, &args.b[seg], full, k0, n0);
-          } else if (GATED) {
-#pragma unroll
-            for (int j = 0; j < BN / 64; ++j)
-              ptx::tma_load_2d(b_dst + j * kFfnAtom, &args.b[j / (BN / 128)], full, n0 + (j % (BN / 128)) * 64, k0);
-          } else {
-#pragma unroll
-            for (int j = 0; j < BN / 64; ++j) ptx::tma_load_2d(b_dst + j * kFfnAtom, &args.b[which], full, n0 + j * 64, k0);
-          }
-          if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
         }
       }
-    }
-  } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      constexpr uint32_t idesc = ptx::idesc_bf16_f32(128, BN, A_MN ? 1 : 0, B_NK ? 0 : 1);
-      uint32_t stage = 0, phase = 0, unit = 0;
-      bool ok = true;
-      for (uint32_t t = blockIdx.x; ok && t < num_tiles; t += gridDim.x, unit += C::NACC) {
-        for (uint32_t kb = 0; ok && kb < num_kb; ++kb) {
-          if (!ptx::mbar_wait(ptx::smem_u32(&bar_full[stage]), phase, abort_p)) { ok = false; break; }
-          ptx::tc_fence_after();
-          const uint32_t a_src = smem_base + stage * C::STAGE, b_src = a_src + C::A_BYTES;
+    } else if (warp == 1) {
+      // ---------------- MMA issuer (the leader CTA) ----------------
+      if (leader && lane == 0) {
+        constexpr uint32_t idesc = ptx::idesc_bf16_f32(128 * CTAS, BN, A_MN ? 1 : 0, B_NK ? 0 : 1);
+        auto multiply = [&](uint32_t stage, uint32_t a, uint32_t slot, bool fresh) {
 #pragma unroll
-          for (int a = 0; a < C::NACC; ++a) {
-            const uint32_t slot = (unit + a) % C::SLOTS;
-            if (kb == 0) {  // the epilogue must have drained this accumulator
-              if (!ptx::mbar_wait(ptx::smem_u32(&bar_acc_empty[slot]), (((unit + a) / C::SLOTS) & 1u) ^ 1u, abort_p)) { ok = false; break; }
-              ptx::tc_fence_after();
-            }
+          for (int kk = 0; kk < KPS; ++kk) {
+            const uint32_t a_src = smem_base + stage * C::STAGE + kk * C::BLOCK + a * 2 * kFfnAtom;
+            const uint32_t b_src = smem_base + stage * C::STAGE + kk * C::BLOCK + C::A_BYTES;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               // K-major: rows of 128 bytes in groups of eight 1024 B apart, a step of 16 k is 32 B inside the row.
               // MN-major: atoms of 64 x 64 kFfnAtom apart, groups of eight k rows 1024 B apart, a step is 16 k rows.
-              const uint64_t adesc = A_MN ? ptx::smem_desc_sw128(a_src + a * 2 * kFfnAtom + k * 2048, kFfnAtom, 1024)
-                                          : ptx::smem_desc_sw128(a_src + a * (128 * 128) + k * 32, 16, 1024);
+              const uint64_t adesc = A_MN ? ptx::smem_desc_sw128(a_src + k * 2048, kFfnAtom, 1024)
+                                          : ptx::smem_desc_sw128(a_src + k * 32, 16, 1024);
               const uint64_t bdesc = B_NK ? ptx::smem_desc_sw128(b_src + k * 32, 16, 1024)
                                           : ptx::smem_desc_sw128(b_src + k * 2048, kFfnAtom, 1024);
-              ptx::mma_bf16(tmem_base + slot * BN, adesc, bdesc, idesc, (kb | static_cast<uint32_t>(k)) != 0u);
+              const uint32_t more = fresh && kk == 0 && k == 0 ? 0u : 1u;
+              if (PAIR) ptx::mma_bf16_pair(tmem_base + slot * BN, adesc, bdesc, idesc, more);
+              else ptx::mma_bf16(tmem_base + slot * BN, adesc, bdesc, idesc, more);
             }
-            if (kb + 1 == num_kb) ptx::mma_commit(ptx::smem_u32(&bar_acc_full[slot]));  // this accumulator is complete
           }
-          if (!ok) break;
-          ptx::mma_commit(ptx::smem_u32(&bar_empty[stage]));
-          if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+        };
+        auto commit = [&](uint64_t* bar) {
+          if (PAIR) ptx::mma_commit_pair(ptx::smem_u32(bar), 3);  // on both CTAs' barriers
+          else ptx::mma_commit(ptx::smem_u32(bar));
+        };
+        uint32_t stage = 0, phase = 0, unit = 0;
+        bool ok = true;
+        for (uint32_t t = first; ok && num_st > 0 && t < num_tiles; t += step, unit += NACC) {
+          // The first accumulator's products of the tile's first stages go out before the second accumulator is waited
+          // for: the epilogue hands that one back a few thousand cycles later.
+          const uint32_t ahead = NACC > 1 ? (num_st < C::STAGES ? num_st : C::STAGES) : 0u;
+#pragma unroll
+          for (int a = 0; a < NACC; ++a) {
+            const uint32_t slot = (unit + a) % C::SLOTS;
+            uint32_t s2 = stage, p2 = phase;
+            // the epilogue must have drained this accumulator
+            ok = ok && ptx::mbar_wait_parked(ptx::smem_u32(&bar_acc_empty[slot]), (((unit + a) / C::SLOTS) & 1u) ^ 1u, abort_p);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            for (uint32_t st = 0; st < ahead; ++st) {
+              if (a == 0) {
+                if (!ptx::mbar_wait_parked(ptx::smem_u32(&bar_full[s2]), p2, abort_p)) { ok = false; break; }
+                ptx::tc_fence_after();
+              }
+              multiply(s2, a, slot, st == 0);
+              if (a == NACC - 1) commit(&bar_empty[s2]);
+              if (++s2 == C::STAGES) { s2 = 0; p2 ^= 1u; }
+            }
+            if (!ok) break;
+            if (ahead > 0 && ahead == num_st) commit(&bar_acc_full[slot]);
+            if (a == NACC - 1) {
+              stage = s2;
+              phase = p2;
+            }
+          }
+          for (uint32_t st = ahead; ok && st < num_st; ++st) {
+            if (!ptx::mbar_wait_parked(ptx::smem_u32(&bar_full[stage]), phase, abort_p)) { ok = false; break; }
+            ptx::tc_fence_after();
+#pragma unroll
+            for (int a = 0; a < NACC; ++a) {
+              const uint32_t slot = (unit + a) % C::SLOTS;
+              multiply(stage, a, slot, NACC == 1 && st == 0);
+              if (NACC > 1 && st + 1 == num_st) commit(&bar_acc_full[slot]);  // this accumulator is complete
+            }
+            commit(&bar_empty[stage]);
+            if (NACC == 1 && st + 1 == num_st) commit(&bar_acc_full[unit % C::SLOTS]);
+            if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+          }
         }
       }
     }
   } else {
-    // ---------------- epilogue ----------------
-    const int e = warp - 2;
+    ptx::setmaxnreg_inc<224>();
+    // ---------------- epilogue (every CTA drains its own rows) ----------------
+    const int e = warp - 4;
     const uint32_t quad = static_cast<uint32_t>(warp) & 3u;  // the TMEM lanes a warp may read: 32 * (warp % 4)
     const uint32_t half = static_cast<uint32_t>(e) >> 2;
     constexpr int NB = BN / 64;              // register blocks of 32 columns per warp and accumulator
@@ -204,11 +272,6 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
     uint32_t unit = 0, nstore = 0;
     bool ok = true;
 
-    // Column (inside the accumulator) of register block q of this warp.
-    auto block_col = [&](int q) -> uint32_t {
-      if (GATED) return (q < OB ? 0u : BN / 2u) + half * (BN / 4) + (q < OB ? q : q - OB) * 32u;
-      return half * (BN / 2) + q * 32u;
-    };
     // 32 rows x 32 columns, packed bf16 pairs, to global memory through the staging buffer whose turn it is.
     auto put_box = [&](const uint32_t (&w)[16], const CUtensorMap* map, uint32_t row0, uint32_t col0) {
       const uint32_t buf = stage_box + (nstore & 1u) * kFfnStageBox;
@@ -226,9 +289,19 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
         ptx::tma_store_commit();
       }
     };
-    auto pack = [](float lo, float hi) -> uint32_t {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    auto pack = [](uint32_t lo, uint32_t hi) -> uint32_t {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(lo), __uint_as_float(hi));
       return *reinterpret_cast<const uint32_t*>(&h);
+    };
+    auto add_bias = [&](uint32_t (&r)[32], const float* b) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(b + j);
+        r[j] = __float_as_uint(__uint_as_float(r[j]) + q.x);
+        r[j + 1] = __float_as_uint(__uint_as_float(r[j + 1]) + q.y);
+        r[j + 2] = __float_as_uint(__uint_as_float(r[j + 2]) + q.z);
+        r[j + 3] = __float_as_uint(__uint_as_float(r[j + 3]) + q.w);
+      }
     };
     // The residual of one box: this lane's row, 32 columns.
     auto load_residual = [&](uint4 (&q)[4], uint32_t row, uint32_t col0) {
@@ -236,45 +309,65 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
       for (int v = 0; v < 4; ++v) {
         q[v] = make_uint4(0u, 0u, 0u, 0u);
         if (row < M && col0 + v * 8 < N)
-          q[v] = __ldcs(reinterpret_cast<const uint4*>(args.residual + static_cast<size_t>(row) * N + col0 + v * 8));
+          q[v] = *reinterpret_cast<const uint4*>(args.residual + static_cast<size_t>(row) * N + col0 + v * 8);
       }
     };
 
-    for (uint32_t t = blockIdx.x; t < num_tiles; t += gridDim.x, unit += C::NACC) {
+    for (uint32_t t = first; t < num_tiles; t += step, unit += NACC) {
       const uint32_t which = FORM == kFfnDw && t >= tiles_one ? 1u : 0u;
       const FfnCoord tc = ffn_coord(t - which * tiles_one, tiles_m, tiles_n1);
-      if (EPILOGUE && args.bias[0] != nullptr) {
+      const bool have_bias = EPILOGUE && args.bias[0] != nullptr;
+      const bool have_res = FORM == kFfnFwd && args.residual != nullptr;
+      if (have_bias) {
         // The tile's bias to shared memory while the K loop runs. No warp leaves this loop early, also after a wait has
         // given up: the barriers need all of them.
         ptx::named_bar_sync(1, kFfnEpiWarps * 32);  // every warp has finished with the previous tile's values
-        const uint32_t et = threadIdx.x - 64u;
+        const uint32_t et = threadIdx.x - 128u;
         if (et < BN) {
           const uint32_t side = GATED && et >= TN ? 1u : 0u, col = tc.n * TN + et - side * TN;
           bias_s[et] = col < N ? __ldg(args.bias[side] + col) : 0.0f;
         }
         ptx::named_bar_sync(1, kFfnEpiWarps * 32);
       }
-      const bool have_bias = EPILOGUE && args.bias[0] != nullptr;
-      const bool have_res = FORM == kFfnFwd && args.residual != nullptr;
-      const uint32_t row_a = tc.m * BM + quad * 32, out_col = tc.n * TN + half * (TN / 2);
-      uint4 res[4], res_next[4];
-      if (have_res && ok) load_residual(res_next, row_a + lane, out_col);
-
-      uint32_t r[NB][32];
-      auto acc_addr = [&](uint32_t a) { return tmem_base + ((quad * 32u) << 16) + ((unit + a) % C::SLOTS) * BN; };
-      auto wait_acc = [&](uint32_t a) {
-        if (ok && !ptx::mbar_wait(ptx::smem_u32(&bar_acc_full[(unit + a) % C::SLOTS]), ((unit + a) / C::SLOTS) & 1u, abort_p)) ok = false;
+      const uint32_t row_t = tc.m * C::BM + rank * 128 + quad * 32, out_col = tc.n * TN + half * (TN / 2);
+      // Block q of this warp: result columns out_col + 32 q; its accumulator columns (Gated: of gate, of up).
+      auto acc_addr = [&](int a, int q) {
+        const uint32_t col = GATED ? (q < OB ? 0u : static_cast<uint32_t>(TN)) + half * (TN / 2) + (q < OB ? q : q - OB) * 32u
+                                   : half * (TN / 2) + q * 32u;
+        return tmem_base + ((quad * 32u) << 16) + ((unit + a) % C::SLOTS) * BN + col;
+      };
+      auto wait_acc = [&](int a) {
+        if (ok && !ptx::mbar_wait_parked(ptx::smem_u32(&bar_acc_full[(unit + a) % C::SLOTS]), ((unit + a) / C::SLOTS) & 1u, abort_p)) ok = false;
         ptx::tc_fence_after();
       };
-      auto release_acc = [&](uint32_t a) {
+      auto release_acc = [&](int a) {
         ptx::tc_fence_before();
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bar_acc_empty[(unit + a) % C::SLOTS]));
+        if (lane == 0) {
+          const uint32_t bar = ptx::smem_u32(&bar_acc_empty[(unit + a) % C::SLOTS]);
+          if (PAIR) ptx::mbar_arrive_cluster(ptx::mapa(bar, 0));
+          else ptx::mbar_arrive(bar);
+        }
       };
-      if (num_kb > 0) {
+      uint4 res[4];
+      if (have_res) {
+        // this warp's share of the tile's residual on its way to L2 while the K loop runs: a lane's row is 2 KB and more
+        // from its neighbour's, so a load from HBM per box would be a full latency each (8192^3 with gelu, residual and
+        // stored projections: 1,170 -> see the launcher)
+#pragma unroll
+        for (int a = 0; a < NACC; ++a) {
+          const uint32_t row = row_t + a * 128 * CTAS + lane;
+          if (row < M && out_col < N)
+            ptx::prefetch_l2(args.residual + static_cast<size_t>(row) * N + out_col, min(static_cast<uint32_t>(TN / 2), N - out_col) * 2u);
+        }
+        load_residual(res, row_t + lane, out_col);
+      }
+      uint32_t r[NB][32];
+      if (num_st > 0) {
         wait_acc(0);
         if (!ok) continue;
+        // the whole share of the first accumulator into registers: it is handed back before anything is computed
 #pragma unroll
-        for (int q = 0; q < NB; ++q) ptx::tmem_ld_32x32(acc_addr(0) + block_col(q), r[q]);
+        for (int q = 0; q < NB; ++q) ptx::tmem_ld_32x32(acc_addr(0, q), r[q]);
 #pragma unroll
         for (int q = 0; q < NB; ++q) ptx::tmem_ld_wait_for(r[q]);
         release_acc(0);
@@ -285,77 +378,67 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
           for (int j = 0; j < 32; ++j) r[q][j] = 0u;
       }
 #pragma unroll
-      for (int a = 0; a < C::NACC; ++a) {
-        const uint32_t row0 = row_a + a * 128;
-        if (a > 0 && num_kb > 0) {
+      for (int a = 0; a < NACC; ++a) {
+        const uint32_t row0 = row_t + a * 128 * CTAS;
+        if (a > 0 && num_st > 0) {
 #pragma unroll
           for (int q = 0; q < NB; ++q) ptx::tmem_ld_wait_for(r[q]);
           release_acc(a);
         }
 #pragma unroll
         for (int q = 0; q < OB; ++q) {
+          constexpr int up = GATED ? OB : 0;
           const uint32_t col0 = out_col + q * 32;
           uint32_t w[16];
-          if (!EPILOGUE) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = pack(__uint_as_float(r[q][2 * j]), __uint_as_float(r[q][2 * j + 1]));
-          } else {
-            if (have_res) {
-#pragma unroll
-              for (int v = 0; v < 4; ++v) res[v] = res_next[v];
-              // the next box's residual is under way while this one is computed
-              if (q + 1 < OB) load_residual(res_next, row0 + lane, col0 + 32);
-              else if (a + 1 < C::NACC) load_residual(res_next, row0 + 128 + lane, out_col);
-            }
+          if constexpr (EPILOGUE) {
             if (have_bias) {
-#pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                const float4 b0 = *reinterpret_cast<const float4*>(bias_s + block_col(q) + j);
-                r[q][j] = __float_as_uint(__uint_as_float(r[q][j]) + b0.x);
-                r[q][j + 1] = __float_as_uint(__uint_as_float(r[q][j + 1]) + b0.y);
-                r[q][j + 2] = __float_as_uint(__uint_as_float(r[q][j + 2]) + b0.z);
-                r[q][j + 3] = __float_as_uint(__uint_as_float(r[q][j + 3]) + b0.w);
-                if (GATED) {
-                  constexpr int up = GATED ? OB : 0;
-                  const float4 b1 = *reinterpret_cast<const float4*>(bias_s + block_col(up + q) + j);
-                  r[up + q][j] = __float_as_uint(__uint_as_float(r[up + q][j]) + b1.x);
-                  r[up + q][j + 1] = __float_as_uint(__uint_as_float(r[up + q][j + 1]) + b1.y);
-                  r[up + q][j + 2] = __float_as_uint(__uint_as_float(r[up + q][j + 2]) + b1.z);
-                  r[up + q][j + 3] = __float_as_uint(__uint_as_float(r[up + q][j + 3]) + b1.w);
-                }
-              }
+              add_bias(r[q], bias_s + half * (TN / 2) + q * 32);
+              if constexpr (GATED) add_bias(r[up + q], bias_s + TN + half * (TN / 2) + q * 32);
             }
             if (args.save) {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) w[j] = pack(__uint_as_float(r[q][2 * j]), __uint_as_float(r[q][2 * j + 1]));
+              for (int j = 0; j < 16; ++j) w[j] = pack(r[q][2 * j], r[q][2 * j + 1]);
               put_box(w, &args.z[0], row0, col0);
-              if (GATED) {
-                constexpr int up = GATED ? OB : 0;
+              if constexpr (GATED) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) w[j] = pack(__uint_as_float(r[up + q][2 * j]), __uint_as_float(r[up + q][2 * j + 1]));
+                for (int j = 0; j < 16; ++j) w[j] = pack(r[up + q][2 * j], r[up + q][2 * j + 1]);
                 put_box(w, &args.z[1], row0, col0);
               }
             }
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float f0 = act_value<ACT>(__uint_as_float(r[q][2 * j])), f1 = act_value<ACT>(__uint_as_float(r[q][2 * j + 1]));
-              if (GATED) {
-                constexpr int up = GATED ? OB : 0;
-                f0 *= __uint_as_float(r[up + q][2 * j]);
-                f1 *= __uint_as_float(r[up + q][2 * j + 1]);
-              } else if (have_res) {
-                const uint32_t p = j % 4 == 0 ? res[j / 4].x : j % 4 == 1 ? res[j / 4].y : j % 4 == 2 ? res[j / 4].z : res[j / 4].w;
-                f0 += __uint_as_float(p << 16);
-                f1 += __uint_as_float(p & 0xffff0000u);
+            for (int j0 = 0; j0 < 32; j0 += 8) {
+              float f[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(r[q][j0 + j]);
+              act_values<ACT>(f);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                if constexpr (GATED) f[j] *= __uint_as_float(r[up + q][j0 + j]);
+                r[q][j0 + j] = __float_as_uint(f[j]);
               }
-              w[j] = pack(f0, f1);
+            }
+            if (have_res) {
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                const uint32_t p[4] = {res[v].x, res[v].y, res[v].z, res[v].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  r[q][v * 8 + 2 * j] = __float_as_uint(__uint_as_float(r[q][v * 8 + 2 * j]) + __uint_as_float(p[j] << 16));
+                  r[q][v * 8 + 2 * j + 1] = __float_as_uint(__uint_as_float(r[q][v * 8 + 2 * j + 1]) + __uint_as_float(p[j] & 0xffff0000u));
+                }
+              }
+              // the next box's is under way while this one is stored
+              if (q + 1 < OB) load_residual(res, row0 + lane, col0 + 32);
+              else if (a + 1 < NACC) load_residual(res, row0 + 128 * CTAS + lane, out_col);
             }
           }
-          if (a + 1 < C::NACC && num_kb > 0) {  // this block's registers are free: refill them from the next accumulator
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[j] = pack(r[q][2 * j], r[q][2 * j + 1]);
+          if (a + 1 < NACC && num_st > 0) {  // this block's registers are free: refill them from the next accumulator
             if (q == 0) wait_acc(a + 1);
             if (ok) {
-              ptx::tmem_ld_32x32(acc_addr(a + 1) + block_col(q), r[q]);
-              if (GATED) ptx::tmem_ld_32x32(acc_addr(a + 1) + block_col(OB + q), r[GATED ? OB + q : q]);
+              ptx::tmem_ld_32x32(acc_addr(a + 1, q), r[q]);
+              if constexpr (GATED) ptx::tmem_ld_32x32(acc_addr(a + 1, up + q), r[up + q]);
             }
           }
           put_box(w, &args.c[which], row0, col0);
@@ -368,20 +451,29 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
 
   ptx::tc_fence_before();
   __syncthreads();
+  if (PAIR) {  // neither CTA may exit or free TMEM while the other can still signal it or read its shared memory
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+  }
   if (warp == 1) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem_base, 512);
+    if (PAIR) ptx::tmem_dealloc_pair(tmem_base, 512);
+    else ptx::tmem_dealloc(tmem_base, 512);
   }
   if (threadIdx.x == 0 && abort_flag != 0) g_ffn_status = 1;
 }
 
-// The kernel of a form, an activation and a tile shape (0: 256 x 256, 1: 128 x 256, 2: 128 x 128).
+// The kernel of a form, an activation and a tile shape.
+template <int FORM, int ACT, int CTAS, int NACC, int BN, int KPS>
+FfnKernel ffn_kernel_shape() {
+  return {reinterpret_cast<const void*>(ffn_gemm_kernel<FORM, ACT, CTAS, NACC, BN, KPS>), FfnTile<CTAS, NACC, BN, KPS>::SMEM, read_status};
+}
 template <int FORM, int ACT>
 FfnKernel ffn_kernel_of(int shape) {
   switch (shape) {
-    case 0: return {reinterpret_cast<const void*>(ffn_gemm_kernel<FORM, ACT, 256, 256>), FfnTile<256, 256>::SMEM, read_status};
-    case 1: return {reinterpret_cast<const void*>(ffn_gemm_kernel<FORM, ACT, 128, 256>), FfnTile<128, 256>::SMEM, read_status};
-    default: return {reinterpret_cast<const void*>(ffn_gemm_kernel<FORM, ACT, 128, 128>), FfnTile<128, 128>::SMEM, read_status};
+    case 0: return ffn_kernel_shape<FORM, ACT, 2, 2, 256, 1>();
+    case 1: return ffn_kernel_shape<FORM, ACT, 2, 1, 256, 2>();
+    default: return ffn_kernel_shape<FORM, ACT, 1, 1, 128, 1>();
   }
 }
 

@@ -8,6 +8,7 @@ asynchronous on the given (or current) torch stream.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Sequence
 
 import torch
@@ -415,22 +416,72 @@ def _act_code(act: str, allowed: Sequence[str]) -> int:
     return _ACTS[act]
 
 
-def _allocating(stream: Optional[torch.cuda.Stream]):
-    """Tensors made inside belong to the stream the call runs on: memory that another stream may still be using is not
-    handed out for them, and a workspace that is dropped on return is not handed on before the call's work is done."""
-    return _ALREADY_CURRENT if stream is None else torch.cuda.stream(stream)
+# A tcab_tensor as bytes: what ctypes hands over as a pointer without building a structure field by field (the operators
+# below take five to eleven tensors; building ctypes structures was half of a small call's host time, 24 us of a
+# layernorm_rows_stats call against 12 with packed views).
+_PACK = {1: struct.Struct("<QiII12x").pack, 2: struct.Struct("<QiIII8x").pack, 3: struct.Struct("<QiIIII4x").pack,
+         4: struct.Struct("<QiIIIII").pack}
 
 
-def _ref(t: Optional[torch.Tensor], name: str):
-    return None if t is None else C.byref(_view(t, name))
+def _packed(t: torch.Tensor, name: str, dev: int) -> bytes:
+    """_view as bytes, for a tensor that has to live on device `dev` (the first operand's)."""
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous():
+        code, shape = _DTYPES.get(t.dtype), t.shape
+        if code is not None and 0 < t.numel() < _TWO32 and len(shape) in _PACK:
+            if t.get_device() != dev:
+                raise ValueError(f"{name} is on {t.device} but the first operand is on cuda:{dev}")
+            return _PACK[len(shape)](t.data_ptr(), code, len(shape), *shape)
+    v = _view(t, name)  # refuses what is not a tensor this library takes; empty tensors come through
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device} but the first operand is on cuda:{dev}")
+    return bytes(v)
 
 
-def _workspace(nbytes: int, ref: torch.Tensor) -> Optional[torch.Tensor]:
-    return torch.empty(nbytes, device=ref.device, dtype=torch.uint8) if nbytes else None
+def _packed_opt(t: Optional[torch.Tensor], name: str, dev: int) -> Optional[bytes]:
+    return None if t is None else _packed(t, name, dev)
 
 
-def _ptr(ws: Optional[torch.Tensor]):
-    return C.c_void_p(ws.data_ptr() if ws is not None else 0)
+def _device_of(t: torch.Tensor, name: str) -> int:
+    """The device index of a call's first operand."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _view(t, name)  # raises
+    return t.get_device()
+
+
+class _At:
+    """The device, and for allocations the stream, that a call runs on. Tensors made inside belong to that stream: memory
+    that another stream may still be using is not handed out for them, and a workspace that is dropped on return is not
+    handed on before the call's work is done."""
+
+    __slots__ = ("managers",)
+
+    def __init__(self, dev: int, stream: Optional[torch.cuda.Stream]):
+        self.managers = [torch.cuda.device(dev)] + ([] if stream is None else [torch.cuda.stream(stream)])
+
+    def __enter__(self):
+        for m in self.managers:
+            m.__enter__()
+
+    def __exit__(self, *exc):
+        for m in reversed(self.managers):
+            m.__exit__(*exc)
+        return False
+
+
+def _at(dev: int, stream: Optional[torch.cuda.Stream]):
+    if stream is None and dev == torch._C._cuda_getDevice():
+        return _ALREADY_CURRENT
+    return _At(dev, stream)
+
+
+def _raw_stream(stream: Optional[torch.cuda.Stream], dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+
+
+def _matrices(a: torch.Tensor, an: str, b: torch.Tensor, bn: str) -> None:
+    for t, name in ((a, an), (b, bn)):
+        if not isinstance(t, torch.Tensor) or t.dim() != 2:
+            raise ValueError(f"{name} must be a rank-2 tensor")
 
 
 def layernorm_rows_stats(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps: float = 1e-5,
@@ -438,18 +489,20 @@ def layernorm_rows_stats(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tenso
                          rstd: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> tuple:
     """layernorm_rows that also returns what its backward pass needs: (y, mean, rstd), the statistics fp32 with the
     extents of x without the innermost one (rank-1 x: [1])."""
-    xv = _view(x, "x")
-    with _on_device(x):
-        if out is None or mean is None or rstd is None:
-            with _allocating(stream):
-                shape = x.shape[:-1] or (1,)
-                out = torch.empty_like(x) if out is None else out
-                mean = torch.empty(shape, device=x.device, dtype=torch.float32) if mean is None else mean
-                rstd = torch.empty(shape, device=x.device, dtype=torch.float32) if rstd is None else rstd
-        gv, bv, yv, mv, rv = _view(gamma, "gamma"), _view(beta, "beta"), _view(out, "out"), _view(mean, "mean"), _view(rstd, "rstd")
-        _same_device(("x", x), ("gamma", gamma), ("beta", beta), ("out", out), ("mean", mean), ("rstd", rstd))
-        _lib.check(_lib.load().tcab_layernorm_rows_stats(C.byref(xv), C.byref(gv), C.byref(bv), C.c_float(eps), C.byref(yv),
-                                                         C.byref(mv), C.byref(rv), _stream(stream, x)))
+    dev = _device_of(x, "x")
+    fn = _lib.packed("tcab_layernorm_rows_stats")
+    with _at(dev, stream):
+        xv = _packed(x, "x", dev)
+        if out is None:
+            out = torch.empty_like(x)
+        if mean is None:
+            mean = torch.empty(x.shape[:-1] or (1,), device=x.device, dtype=torch.float32)
+        if rstd is None:
+            rstd = torch.empty(x.shape[:-1] or (1,), device=x.device, dtype=torch.float32)
+        rc = fn(xv, _packed(gamma, "gamma", dev), _packed(beta, "beta", dev), eps, _packed(out, "out", dev),
+                _packed(mean, "mean", dev), _packed(rstd, "rstd", dev), _raw_stream(stream, dev))
+    if rc:
+        _lib.check(rc)
     return out, mean, rstd
 
 
@@ -458,21 +511,23 @@ def layernorm_rows_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tens
                             dbeta: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> tuple:
     """Backward pass of layernorm_rows_stats: (dx, dgamma, dbeta). dx has the type of x (it may be dy or x themselves),
     dgamma and dbeta are fp32."""
-    xv = _view(x, "x")
-    lib = _lib.load()
-    with _on_device(x):
-        with _allocating(stream):
-            cols = x.shape[-1]
-            dx = torch.empty_like(x) if dx is None else dx
-            dgamma = torch.empty(cols, device=x.device, dtype=torch.float32) if dgamma is None else dgamma
-            dbeta = torch.empty(cols, device=x.device, dtype=torch.float32) if dbeta is None else dbeta
-            nbytes = lib.tcab_layernorm_rows_backward_workspace(C.byref(xv))
-            ws = _workspace(nbytes, x)
-        _same_device(("x", x), ("dy", dy), ("gamma", gamma), ("mean", mean), ("rstd", rstd), ("dx", dx), ("dgamma", dgamma),
-                     ("dbeta", dbeta))
-        _lib.check(lib.tcab_layernorm_rows_backward(
-            _ref(dy, "dy"), C.byref(xv), _ref(gamma, "gamma"), _ref(mean, "mean"), _ref(rstd, "rstd"), _ref(dx, "dx"),
-            _ref(dgamma, "dgamma"), _ref(dbeta, "dbeta"), _ptr(ws), nbytes, _stream(stream, x)))
+    dev = _device_of(x, "x")
+    fn, need = _lib.packed("tcab_layernorm_rows_backward"), _lib.packed("tcab_layernorm_rows_backward_workspace")
+    with _at(dev, stream):
+        xv = _packed(x, "x", dev)
+        if dx is None:
+            dx = torch.empty_like(x)
+        if dgamma is None:
+            dgamma = torch.empty(x.shape[-1], device=x.device, dtype=torch.float32)
+        if dbeta is None:
+            dbeta = torch.empty(x.shape[-1], device=x.device, dtype=torch.float32)
+        nbytes = need(xv)
+        ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
+        rc = fn(_packed(dy, "dy", dev), xv, _packed(gamma, "gamma", dev), _packed(mean, "mean", dev), _packed(rstd, "rstd", dev),
+                _packed(dx, "dx", dev), _packed(dgamma, "dgamma", dev), _packed(dbeta, "dbeta", dev),
+                ws.data_ptr() if nbytes else None, nbytes, _raw_stream(stream, dev))
+    if rc:
+        _lib.check(rc)
     return dx, dgamma, dbeta
 
 
@@ -483,29 +538,27 @@ def gemm_bias_act_residual(a: torch.Tensor, b: torch.Tensor, bias: Optional[torc
     none, relu, silu, gelu, gelu_tanh. preact [M,N] bf16, where given, receives a @ b + bias for the backward pass. c may
     be the residual itself (out=residual)."""
     code = _act_code(act, _PLAIN_ACTS)
-    av, bv = _view(a, "a"), _view(b, "b")
-    if av.rank != 2 or bv.rank != 2:
-        raise ValueError("a and b must be rank 2")
-    with _on_device(a):
+    dev = _device_of(a, "a")
+    _matrices(a, "a", b, "b")
+    fn = _lib.packed("tcab_gemm_bias_act_residual")
+    with _at(dev, stream):
         if out is None:
-            with _allocating(stream):
-                out = torch.empty((a.shape[0], b.shape[1]), device=a.device, dtype=torch.bfloat16)
-        _same_device(("a", a), ("b", b), ("bias", bias), ("residual", residual), ("out", out), ("preact", preact))
-        _lib.check(_lib.load().tcab_gemm_bias_act_residual(
-            C.byref(av), C.byref(bv), _ref(bias, "bias"), _ref(residual, "residual"), code, _ref(preact, "preact"),
-            _ref(out, "out"), _stream(stream, a)))
+            out = torch.empty((a.shape[0], b.shape[1]), device=a.device, dtype=torch.bfloat16)
+        rc = fn(_packed(a, "a", dev), _packed(b, "b", dev), _packed_opt(bias, "bias", dev), _packed_opt(residual, "residual", dev),
+                code, _packed_opt(preact, "preact", dev), _packed(out, "out", dev), _raw_stream(stream, dev))
+    if rc:
+        _lib.check(rc)
     return out
 
 
-def _wanted(want: Sequence[str], known: Sequence[str], out: Optional[dict], shapes: dict, ref: torch.Tensor) -> dict:
+def _wanted(want: Sequence[str], out: Optional[dict], shapes: dict, device: torch.device) -> dict:
     """The outputs a backward pass is to compute, by name: the caller's where given, new ones otherwise."""
-    res = dict(out or {})
-    for name in list(res) + list(want):
-        if name not in known:
-            raise ValueError(f"unknown output {name!r} (one of {', '.join(known)})")
-    for name in want:
+    res = dict(out) if out else {}
+    for name in (*res, *want):
+        if name not in shapes:
+            raise ValueError(f"unknown output {name!r} (one of {', '.join(shapes)})")
         if name not in res:
-            res[name] = torch.empty(shapes[name], device=ref.device,
+            res[name] = torch.empty(shapes[name], device=device,
                                     dtype=torch.float32 if name.startswith("dbias") else torch.bfloat16)
     return res
 
@@ -516,20 +569,20 @@ def gemm_bias_act_backward(dc: torch.Tensor, a: torch.Tensor, b: torch.Tensor, p
     """Backward pass of gemm_bias_act_residual; returns {"da" [M,K] bf16, "db" [K,N] bf16, "dbias" [N] fp32} as requested
     (the gradient of the residual is dc). preact is what the forward pass stored; it is not needed for act="none"."""
     code = _act_code(act, _PLAIN_ACTS)
-    av, bv = _view(a, "a"), _view(b, "b")
-    if av.rank != 2 or bv.rank != 2:
-        raise ValueError("a and b must be rank 2")
-    m, k, n = a.shape[0], a.shape[1], b.shape[1]
-    lib = _lib.load()
-    with _on_device(a):
-        with _allocating(stream):
-            res = _wanted(want, ("da", "db", "dbias"), out, {"da": (m, k), "db": (k, n), "dbias": (n,)}, a)
-            nbytes = lib.tcab_gemm_bias_act_backward_workspace(m, n, code, int("dbias" in res))
-            ws = _workspace(nbytes, a)
-        _same_device(("a", a), ("b", b), ("dc", dc), ("preact", preact), *res.items())
-        _lib.check(lib.tcab_gemm_bias_act_backward(
-            _ref(dc, "dc"), C.byref(av), C.byref(bv), _ref(preact, "preact"), code, _ref(res.get("da"), "da"),
-            _ref(res.get("db"), "db"), _ref(res.get("dbias"), "dbias"), _ptr(ws), nbytes, _stream(stream, a)))
+    dev = _device_of(a, "a")
+    _matrices(a, "a", b, "b")
+    (m, k), n = a.shape, b.shape[1]
+    fn, need = _lib.packed("tcab_gemm_bias_act_backward"), _lib.packed("tcab_gemm_bias_act_backward_workspace")
+    with _at(dev, stream):
+        av, bv = _packed(a, "a", dev), _packed(b, "b", dev)
+        res = _wanted(want, out, {"da": (m, k), "db": (k, n), "dbias": (n,)}, a.device)
+        nbytes = need(m, n, code, "dbias" in res)
+        ws = torch.empty(nbytes, device=a.device, dtype=torch.uint8) if nbytes else None
+        rc = fn(_packed(dc, "dc", dev), av, bv, _packed_opt(preact, "preact", dev), code, _packed_opt(res.get("da"), "da", dev),
+                _packed_opt(res.get("db"), "db", dev), _packed_opt(res.get("dbias"), "dbias", dev),
+                ws.data_ptr() if nbytes else None, nbytes, _raw_stream(stream, dev))
+    if rc:
+        _lib.check(rc)
     return res
 
 
@@ -541,18 +594,17 @@ def gated_gemm(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, bias_g
     the biases [N] fp32 (both or neither); act one of silu, gelu, gelu_tanh, sigmoid, relu. gate and up [M,N] bf16 (both or
     neither) receive the two projections for the backward pass."""
     code = _act_code(act, _GATE_ACTS)
-    xv, gv = _view(x, "x"), _view(w_gate, "w_gate")
-    if xv.rank != 2 or gv.rank != 2:
-        raise ValueError("x and w_gate must be rank 2")
-    with _on_device(x):
+    dev = _device_of(x, "x")
+    _matrices(x, "x", w_gate, "w_gate")
+    fn = _lib.packed("tcab_gated_gemm")
+    with _at(dev, stream):
         if out is None:
-            with _allocating(stream):
-                out = torch.empty((x.shape[0], w_gate.shape[1]), device=x.device, dtype=torch.bfloat16)
-        _same_device(("x", x), ("w_gate", w_gate), ("w_up", w_up), ("bias_gate", bias_gate), ("bias_up", bias_up), ("out", out),
-                     ("gate", gate), ("up", up))
-        _lib.check(_lib.load().tcab_gated_gemm(
-            C.byref(xv), C.byref(gv), _ref(w_up, "w_up"), _ref(bias_gate, "bias_gate"), _ref(bias_up, "bias_up"), code,
-            _ref(gate, "gate"), _ref(up, "up"), _ref(out, "out"), _stream(stream, x)))
+            out = torch.empty((x.shape[0], w_gate.shape[1]), device=x.device, dtype=torch.bfloat16)
+        rc = fn(_packed(x, "x", dev), _packed(w_gate, "w_gate", dev), _packed(w_up, "w_up", dev),
+                _packed_opt(bias_gate, "bias_gate", dev), _packed_opt(bias_up, "bias_up", dev), code, _packed_opt(gate, "gate", dev),
+                _packed_opt(up, "up", dev), _packed(out, "out", dev), _raw_stream(stream, dev))
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -562,21 +614,18 @@ def gated_gemm_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor,
     """Backward pass of gated_gemm from the projections it stored; returns {"dx" [M,K], "dw_gate" and "dw_up" [K,N] bf16,
     "dbias_gate" and "dbias_up" [N] fp32} as requested (the weights' gradients both or neither, the biases' likewise)."""
     code = _act_code(act, _GATE_ACTS)
-    xv, gv = _view(x, "x"), _view(w_gate, "w_gate")
-    if xv.rank != 2 or gv.rank != 2:
-        raise ValueError("x and w_gate must be rank 2")
-    m, k, n = x.shape[0], x.shape[1], w_gate.shape[1]
-    known = {"dx": (m, k), "dw_gate": (k, n), "dw_up": (k, n), "dbias_gate": (n,), "dbias_up": (n,)}
-    lib = _lib.load()
-    with _on_device(x):
-        with _allocating(stream):
-            res = _wanted(want, tuple(known), out, known, x)
-            nbytes = lib.tcab_gated_gemm_backward_workspace(m, n, int("dbias_gate" in res or "dbias_up" in res))
-            ws = _workspace(nbytes, x)
-        _same_device(("x", x), ("w_gate", w_gate), ("w_up", w_up), ("dh", dh), ("gate", gate), ("up", up), *res.items())
-        _lib.check(lib.tcab_gated_gemm_backward(
-            _ref(dh, "dh"), C.byref(xv), C.byref(gv), _ref(w_up, "w_up"), _ref(gate, "gate"), _ref(up, "up"), code,
-            _ref(res.get("dx"), "dx"), _ref(res.get("dw_gate"), "dw_gate"), _ref(res.get("dw_up"), "dw_up"),
-            _ref(res.get("dbias_gate"), "dbias_gate"), _ref(res.get("dbias_up"), "dbias_up"), _ptr(ws), nbytes,
-            _stream(stream, x)))
+    dev = _device_of(x, "x")
+    _matrices(x, "x", w_gate, "w_gate")
+    (m, k), n = x.shape, w_gate.shape[1]
+    fn, need = _lib.packed("tcab_gated_gemm_backward"), _lib.packed("tcab_gated_gemm_backward_workspace")
+    with _at(dev, stream):
+        xv, gv = _packed(x, "x", dev), _packed(w_gate, "w_gate", dev)
+        res = _wanted(want, out, {"dx": (m, k), "dw_gate": (k, n), "dw_up": (k, n), "dbias_gate": (n,), "dbias_up": (n,)}, x.device)
+        nbytes = need(m, n, "dbias_gate" in res or "dbias_up" in res)
+        ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
+        rc = fn(_packed(dh, "dh", dev), xv, gv, _packed(w_up, "w_up", dev), _packed(gate, "gate", dev), _packed(up, "up", dev), code,
+                *[_packed_opt(res.get(name), name, dev) for name in ("dx", "dw_gate", "dw_up", "dbias_gate", "dbias_up")],
+                ws.data_ptr() if nbytes else None, nbytes, _raw_stream(stream, dev))
+    if rc:
+        _lib.check(rc)
     return res

@@ -28,7 +28,7 @@ def ints(*shape, seed, lo=-2, hi=3):
     return torch.randint(lo, hi, shape, device="cuda", generator=g).to(BF)
 
 
-@pytest.fixture(params=[0, 1, 2, 3], ids=["chosen", "256x256", "128x256", "128x128"])
+@pytest.fixture(params=[0, 1, 2, 3], ids=["chosen", "512x256", "256x256", "128x128"])
 def tile(request, tcab_lib):
     import tcacomp_b200 as T
     T.tune("ffn", 0, request.param)
