@@ -366,12 +366,13 @@ uint64_t tcab_launch_count(void) { return g_launches.load(std::memory_order_rela
 int tcab_device_status(int* status) {
   if (status == nullptr) return fail(TCAB_ERR_INVALID_ARG, "device_status: null output");
   TCAB_TRY(have_device("device_status"));
-  int gemm = 0, rows = 0, ffn = 0;
+  int gemm = 0, rows = 0, ffn = 0, norm = 0;
   TCAB_TRY(gemm_device_status(&gemm));
   TCAB_TRY(rows_smem_status(&rows));
   TCAB_TRY(ffn_device_status(&ffn));
-  // 1..5: a kernel of gemm_bias_act.cu, 8: one of ffn_gemm.cuh, 16: a shared-memory row kernel
-  *status = gemm != 0 ? gemm : ffn != 0 ? 8 : (rows != 0 ? 16 : 0);
+  TCAB_TRY(layernorm_backward_status(&norm));
+  // 1..5: a kernel of gemm_bias_act.cu, 8: one of ffn_gemm.cuh, 16: a shared-memory row kernel, 32: ln_bwd_ring
+  *status = gemm != 0 ? gemm : ffn != 0 ? 8 : rows != 0 ? 16 : (norm != 0 ? 32 : 0);
   return TCAB_OK;
 }
 

@@ -109,7 +109,7 @@ act_backward_finish(const float* __restrict__ sum, uint32_t parts, uint32_t ns, 
   const uint64_t c = static_cast<uint64_t>(blockIdx.x) * 32 + lane, width = static_cast<uint64_t>(ns) * cols;
   float t = 0.0f;
   if (c < width) {
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t p = warp; p < parts; p += 8) t += sum[p * width + c];
   }
   meet[warp][lane] = t;

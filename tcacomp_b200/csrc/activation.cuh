@@ -23,57 +23,44 @@
 // the tail form 1,250, eight at a time 1,3xx; without an activation 1,400.
 #pragma once
 
-#include "common.cuh"
+#include "f32x2.cuh"
 
 #ifdef __CUDACC__
 namespace tcab {
-
-// two fp32 values as a register pair
-__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
-  uint64_t p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
-  return p;
-}
-__device__ __forceinline__ void pair_to(uint64_t p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 
 // s = 1 / (1 + exp(-z))
 __device__ __forceinline__ void logistic8(const float (&z)[8], float (&s)[8]) {
   float e[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) e[j] = __expf(-z[j]);
+  for (int j = 0; j < 8; ++j) e[j] = exp2_hw(-1.4426950408889634f * z[j]);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) s[j] = __fdividef(1.0f, 1.0f + e[j]);
+  for (int j = 0; j < 8; ++j) s[j] = rcp_hw(1.0f + e[j]);
 }
 
 // e = exp(-z^2 / 2), q = Q(|z|)
 __device__ __forceinline__ void normal_tail8(const float (&z)[8], float (&e)[8], float (&q)[8]) {
   float t[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) t[j] = __fdividef(1.0f, fmaf(0.2316419f, fabsf(z[j]), 1.0f));
+  for (int j = 0; j < 8; ++j) t[j] = rcp_hw(fmaf(0.2316419f, fabsf(z[j]), 1.0f));
 #pragma unroll
-  for (int j = 0; j < 8; ++j) e[j] = __expf(-0.5f * z[j] * z[j]);
-  uint64_t tp[4], p[4];
+  for (int j = 0; j < 4; ++j) {  // -z^2 / 2 in units of ln 2
+    const f32x2 zp = pair_of(z[2 * j], z[2 * j + 1]);
+    pair_to(mul_pair(mul_pair(zp, spread<f32x2>(-0.7213475204444817f)), zp), e[2 * j], e[2 * j + 1]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) e[j] = exp2_hw(e[j]);
+  f32x2 tp[4], p[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     tp[j] = pair_of(t[2 * j], t[2 * j + 1]);
-    p[j] = fma_pair(tp[j], pair_of(0.5307027143f, 0.5307027143f), pair_of(-0.7265760131f, -0.7265760131f));
+    p[j] = fma_pair(tp[j], spread<f32x2>(0.5307027143f), spread<f32x2>(-0.7265760131f));
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) p[j] = fma_pair(tp[j], p[j], pair_of(0.7107068707f, 0.7107068707f));
+  for (int j = 0; j < 4; ++j) p[j] = fma_pair(tp[j], p[j], spread<f32x2>(0.7107068707f));
 #pragma unroll
-  for (int j = 0; j < 4; ++j) p[j] = fma_pair(tp[j], p[j], pair_of(-0.1422483683f, -0.1422483683f));
+  for (int j = 0; j < 4; ++j) p[j] = fma_pair(tp[j], p[j], spread<f32x2>(-0.1422483683f));
 #pragma unroll
-  for (int j = 0; j < 4; ++j) p[j] = fma_pair(tp[j], p[j], pair_of(0.1274147959f, 0.1274147959f));
+  for (int j = 0; j < 4; ++j) p[j] = fma_pair(tp[j], p[j], spread<f32x2>(0.1274147959f));
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     p[j] = mul_pair(p[j], mul_pair(tp[j], pair_of(e[2 * j], e[2 * j + 1])));

@@ -91,6 +91,7 @@ int launch_layernorm_rows_f32(const float* x, const float* gamma, const float* b
                               float* y, RowStats st, uint64_t rows, uint32_t cols, cudaStream_t s);
 // layernorm_backward.cu; the workspace of a size covers every alignment of its operands
 uint64_t layernorm_backward_workspace(uint64_t rows, uint32_t cols, int elem_bytes);
+int layernorm_backward_status(int* out);
 int launch_layernorm_backward_bf16(const __nv_bfloat16* dy, const __nv_bfloat16* x, const __nv_bfloat16* gamma, const float* mean,
                                    const float* rstd, __nv_bfloat16* dx, float* dgamma, float* dbeta, uint64_t rows, uint32_t cols,
                                    void* ws, uint64_t ws_bytes, cudaStream_t s);
