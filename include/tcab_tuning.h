@@ -43,7 +43,8 @@ extern "C" {
  *       tensor cores; 128: p3 = workspace cap in MiB of the three-piece f32 contraction, which then runs in blocks),
  *       p3 = ranges the K blocks of a tile are cut into by kernels 3, 4 and 5 (1 = no split; 2..8 for 5).
  *   "ffn" (the contractions of tcab_gemm_bias_act_residual, tcab_gated_gemm and their backward passes): p0 = CTAs of
- *       the persistent grid, p1 = tile shape (1 512 x 256 and 2 256 x 256 on a pair of CTAs, 3 128 x 128). */
+ *       the persistent grid, p1 = tile shape (1 512 x 256 and 2 256 x 256 on a pair of CTAs, 3 128 x 128,
+ *       4 a tile per cluster), p3 = CTAs per tile of the last (1..8). */
 TCAB_API int tcab_tune(const char* family, int p0, int p1, int p2, int p3);
 
 

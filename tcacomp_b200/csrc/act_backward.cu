@@ -13,6 +13,7 @@
 #include "activation.cuh"
 #include "ffn_gemm.h"
 #include "rowvec.cuh"
+#include "sm100_ptx.cuh"
 
 namespace tcab {
 namespace {
@@ -29,6 +30,8 @@ act_backward_kernel(const __nv_bfloat16* __restrict__ in0, const __nv_bfloat16* 
                     const __nv_bfloat16* __restrict__ in2, __nv_bfloat16* __restrict__ out0, __nv_bfloat16* __restrict__ out1,
                     float* __restrict__ sum, uint32_t rows, uint32_t cols) {
   constexpr int NS = GATED ? 2 : 1;
+  ptx::pdl_wait();
+  ptx::pdl_launch();
   __shared__ float part[SUMS ? kCtaRows : 1][SUMS ? kStripCols + 8 : 1];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t col = blockIdx.x * kStripCols + lane * 8;
@@ -105,6 +108,8 @@ __global__ void __launch_bounds__(256)
 act_backward_finish(const float* __restrict__ sum, uint32_t parts, uint32_t ns, uint32_t cols, float* __restrict__ out0,
                     float* __restrict__ out1) {
   __shared__ float meet[8][33];
+  ptx::pdl_wait();
+  ptx::pdl_launch();
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t c = static_cast<uint64_t>(blockIdx.x) * 32 + lane, width = static_cast<uint64_t>(ns) * cols;
   float t = 0.0f;
@@ -147,13 +152,14 @@ int launch(const char* op, const __nv_bfloat16* in0, const __nv_bfloat16* in1, c
   float* sum = static_cast<float*>(ws);
   const bool direct = sums && !GATED && parts == 1;  // one partial row: it is the result
   if (direct) sum = dbias0;
-  if (sums) act_backward_kernel<ACT, GATED, true><<<grid, 256, 0, s>>>(in0, in1, in2, out0, out1, sum, rows, cols);
-  else act_backward_kernel<ACT, GATED, false><<<grid, 256, 0, s>>>(in0, in1, in2, out0, out1, nullptr, rows, cols);
+  if (sums) launch_pdl(act_backward_kernel<ACT, GATED, true>, grid, dim3(256), 0, s, in0, in1, in2, out0, out1, sum, rows, cols);
+  else launch_pdl(act_backward_kernel<ACT, GATED, false>, grid, dim3(256), 0, s, in0, in1, in2, out0, out1, static_cast<float*>(nullptr), rows, cols);
   count_launch();
   const int rc = check_launch(op);
   if (rc != TCAB_OK || !sums || direct) return rc;
   const uint32_t ns = GATED ? 2 : 1;
-  act_backward_finish<<<static_cast<unsigned>((static_cast<uint64_t>(ns) * cols + 31) / 32), 256, 0, s>>>(sum, parts, ns, cols, dbias0, dbias1);
+  launch_pdl(act_backward_finish, dim3(static_cast<unsigned>((static_cast<uint64_t>(ns) * cols + 31) / 32)), dim3(256), 0, s,
+             static_cast<const float*>(sum), parts, ns, cols, dbias0, dbias1);
   count_launch();
   return check_launch(op);
 }

@@ -259,6 +259,23 @@ int gemm_device_status(int* out);  // status word of the contraction kernel (syn
 // ---------------------------------------------------------------------------
 #ifdef __CUDACC__
 
+// A launch that may overlap the end of its predecessor on the stream: the kernel waits (ptx::pdl_wait) before it touches
+// global memory. Errors are left for check_launch.
+template <typename... P, typename... A>
+inline void launch_pdl(void (*fn)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, fn, args...);
+}
+
 constexpr unsigned kFullMask = 0xffffffffu;
 
 // 128-bit loads/stores for data that is touched once. The cache policy is a build-time

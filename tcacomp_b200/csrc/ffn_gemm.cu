@@ -44,19 +44,30 @@ FfnKernel kernel_of(int form, int act, int shape) {
 // The tile shapes of ffn_kernel_of.
 constexpr int kShapes = 3, kCtas[kShapes] = {2, 2, 1}, kRows[kShapes] = {512, 256, 128}, kBN[kShapes] = {256, 256, 128};
 
-// The tile shape: fewest rounds over the SMs (pairs of SMs), weighted by what a round of each shape costs.
-int pick_shape(int form, const FfnProblem& p) {
-  static const double kCost[kShapes] = {1.0, 0.55, 0.36};  // of a round of one tile per CTA or pair
-  const uint64_t sms = static_cast<uint64_t>(sm_count()), outs = form == kFfnDw && p.b[1] != nullptr ? 2 : 1;
-  int best = 0;
-  double best_cost = 1e300;
+// The kernel: a tile shape of the persistent one, or kShapes for ffn_small.cuh. An estimate in microseconds per shape --
+// what a launch costs before its first and behind its last block, rounds over the SMs (pairs of SMs), blocks of 64 per
+// round -- fitted to outputs of 1003 x 2728, 1024 x 2816 and 512 x 4096 over 64 ... 2048 (graphs of launches):
+//   512 x 256 on pairs 8.3 + 0.49 per block, 256 x 256 on pairs 5.8 + 0.30, 128 x 128 3.6 + 0.30 (its two operand tiles per
+//   128 x 128 products are at the shared-memory limit), against 3.1-3.7 for a library product's launch.
+// Over many rounds the 512 x 256 tile wins (8192^3: 1,395 TFLOP/s against 1,305 for 256 x 256): it moves the fewest bytes.
+int choose(int form, const FfnProblem& p) {
+  static const double kFixed[kShapes] = {8.3, 5.8, 3.6}, kBlock[kShapes] = {0.49, 0.30, 0.30}, kEpilogue[kShapes] = {4.0, 2.2, 1.0};
+  const uint64_t sms = static_cast<uint64_t>(sm_count());
+  const uint32_t pairs = p.b[1] != nullptr ? 2 : 1;
+  const uint64_t outs = form == kFfnDw ? pairs : 1, blocks = (static_cast<uint64_t>(p.K) + 63) / 64 * (form == kFfnDx ? pairs : 1);
+  int best = kShapes;
+  double best_us = ffn_small_plan(form, p.M, p.N, p.K, pairs, sm_count(), 0).us;
   for (int s = 0; s < kShapes; ++s) {
     const uint64_t bm = kRows[s], tn = static_cast<uint64_t>(form == kFfnGated ? kBN[s] / 2 : kBN[s]);
     const uint64_t tiles = (p.M + bm - 1) / bm * ((p.N + tn - 1) / tn) * outs, at_once = sms / kCtas[s];
     if (at_once == 0) continue;
-    const double cost = static_cast<double>((tiles + at_once - 1) / at_once) * kCost[s];
-    if (cost < best_cost - 1e-9) {
-      best_cost = cost;
+    const uint64_t rounds = (tiles + at_once - 1) / at_once;
+    // a round's end is hidden where two accumulators alternate; the 512 x 256 tile pays part of it every time
+    double round = static_cast<double>(blocks) * kBlock[s] + (s == 0 ? 3.0 : 0.8);
+    if (round < kEpilogue[s]) round = kEpilogue[s];  // few blocks: the time of storing a tile
+    const double us = kFixed[s] + static_cast<double>(rounds) * round;
+    if (us < best_us - 1e-9) {
+      best_us = us;
       best = s;
     }
   }
@@ -67,6 +78,7 @@ int pick_shape(int form, const FfnProblem& p) {
 
 int ffn_device_status(int* out) {
   *out = 0;
+  TCAB_TRY_RC(ffn_small_status(out));
   for (int form = kFfnFwd; form <= kFfnDw; ++form)
     for (int act = TCAB_ACT_NONE; act <= TCAB_ACT_SIGMOID; ++act) {
       if (form >= kFfnDx && act != TCAB_ACT_NONE) continue;
@@ -85,7 +97,8 @@ int ffn_device_status(int* out) {
 int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t s) {
   if (p.M == 0 || p.N == 0) return TCAB_OK;
   const Tune& tn = tune(kFfn);
-  const int shape = tn.p1 > 0 && tn.p1 <= kShapes ? tn.p1 - 1 : pick_shape(form, p);
+  const int shape = tn.p1 > 0 && tn.p1 <= kShapes + 1 ? tn.p1 - 1 : choose(form, p);
+  if (shape == kShapes) return launch_ffn_small(op, form, p, s);
   const uint32_t ctas = kCtas[shape], bm = kRows[shape], bn = kBN[shape], tile_n = form == kFfnGated ? bn / 2 : bn;
   FfnArgs args = {};
   args.M = p.M;
@@ -109,11 +122,10 @@ int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t 
       else TCAB_TRY_RC(make_tensor_map(op, &args.b[i], p.b[i], p.K, p.N, 64, 64));
     }
   }
-  const int nc = form == kFfnDw ? nb : 1;
-  for (int i = 0; i < nc; ++i) TCAB_TRY_RC(make_tensor_map(op, &args.c[i], p.c[i], p.M, p.N, 32, 32));
-  for (int i = 0; i < 2; ++i)
-    if (p.z[i] != nullptr) TCAB_TRY_RC(make_tensor_map(op, &args.z[i], p.z[i], p.M, p.N, 32, 32));
-
+  for (int i = 0; i < 2; ++i) {
+    args.c[i] = p.c[i];
+    args.z[i] = p.z[i];
+  }
   const FfnKernel k = kernel_of(form, p.act, shape);
   if (k.fn == nullptr) return fail(TCAB_ERR_UNSUPPORTED, "%s: no kernel for activation %d", op, p.act);
   const cudaError_t ae = cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(k.smem));
@@ -130,13 +142,15 @@ int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t 
   cfg.blockDim = dim3(kFfnThreads);
   cfg.dynamicSmemBytes = k.smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ctas;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 2;
   void* params[] = {&args};
   const cudaError_t le = cudaLaunchKernelExC(&cfg, k.fn, params);
   count_launch();

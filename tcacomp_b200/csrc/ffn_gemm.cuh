@@ -15,8 +15,10 @@
 // holds 512 / BN of them in a ring, so that the epilogue of a tile -- activations, products, residuals, up to three stored
 // matrices -- runs under the K loop of the next. It takes 32 columns at a time, with the next 32 under way from TMEM.
 //
-// Results leave through 32 x 32 boxes in two alternating staging buffers per warp and TMA stores, which clip ragged
-// edges. Loads past an edge read zeros. Every wait is bounded (sm100_ptx.cuh); a wait that gives up ends the kernel
+// Results leave as 32 x 32 boxes: a lane holds a row of 32 columns, the box turns in a 2 KB buffer of the warp, and four
+// 16-byte stores per lane write 64-byte row segments. (TMA stores from two such buffers were measured first: about 1,000
+// cycles per box, most of them waiting for a buffer to be read, against 250; where a CTA has one tile, nothing hides
+// that.) A residual takes the same way in. Loads past an edge read zeros. Every wait is bounded (sm100_ptx.cuh); a wait that gives up ends the kernel
 // with a status word.
 #pragma once
 
@@ -31,7 +33,9 @@ constexpr int kFfnAtom = kFfnBK * 128;  // a box of 64 x 64 bf16
 constexpr int kFfnStageBox = 32 * 64;   // a box of 32 x 32 bf16 results
 
 struct FfnArgs {
-  CUtensorMap a[2], b[2], c[2], z[2];
+  CUtensorMap a[2], b[2];
+  __nv_bfloat16* c[2];
+  __nv_bfloat16* z[2];
   const float* bias[2];
   const __nv_bfloat16* residual;
   uint32_t M, N, K;
@@ -115,7 +119,12 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
     }
     ptx::fence_barrier_init();
     ptx::fence_proxy_async();
+    ptx::prefetch_tensormap(&args.a[0]);
+    ptx::prefetch_tensormap(&args.b[0]);
+    if (GATED || (FORM >= kFfnDx && args.pairs == 2)) ptx::prefetch_tensormap(&args.b[1]);
   }
+  __syncwarp();
+  if (PAIR) ptx::cluster_arrive();  // this CTA's barriers are initialised
   if (warp == 1) {
     if (PAIR) {
       ptx::tmem_alloc_pair(ptx::smem_u32(&tmem_base_slot), 512);
@@ -127,12 +136,11 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
   }
   ptx::tc_fence_before();
   __syncthreads();
-  if (PAIR) {  // the peer's barriers must be initialised before anything of this CTA can signal them
-    ptx::cluster_arrive();
-    ptx::cluster_wait();
-  }
+  if (PAIR) ptx::cluster_wait();  // the peer's barriers must be initialised before anything of this CTA can signal them
   ptx::tc_fence_after();
   const uint32_t tmem_base = tmem_base_slot;
+  ptx::pdl_wait();
+  ptx::pdl_launch();
 
   // Register split: 384 threads x 168 at launch = 64,512; 128 x 40 + 256 x 224 = 62,464 afterwards.
   if (warp < 4) {
@@ -269,25 +277,24 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
     constexpr int OB = GATED ? NB / 2 : NB;  // result boxes per accumulator (Gated: blocks q and OB + q are gate and up)
     const uint32_t stage_box = smem_base + C::STAGES * C::STAGE + e * 2 * kFfnStageBox;
     const uint32_t sw = (static_cast<uint32_t>(lane) >> 1) & 3u;
-    uint32_t unit = 0, nstore = 0;
+    uint32_t unit = 0;
     bool ok = true;
 
-    // 32 rows x 32 columns, packed bf16 pairs, to global memory through the staging buffer whose turn it is.
-    auto put_box = [&](const uint32_t (&w)[16], const CUtensorMap* map, uint32_t row0, uint32_t col0) {
-      const uint32_t buf = stage_box + (nstore & 1u) * kFfnStageBox;
-      ++nstore;
-      if (lane == 0) ptx::tma_store_wait_read_1();  // the store before the last one has left this buffer
-      __syncwarp();
-      const uint32_t my_row = buf + static_cast<uint32_t>(lane) * 64u;
+    // This lane's place in a turned box: rows lane / 4 + 8 i, the 16-byte chunk lane % 4 of their 64 bytes.
+    const uint32_t trow = static_cast<uint32_t>(lane) >> 2, tchunk = static_cast<uint32_t>(lane) & 3u;
+    const uint32_t my_row = stage_box + static_cast<uint32_t>(lane) * 64u;
+    auto turned = [&](uint32_t i) { return (trow + 8 * i) * 64u + ((tchunk ^ (((trow + 8 * i) >> 1) & 3u)) * 16u); };
+    // 32 rows x 32 columns, packed bf16 pairs, to global memory.
+    auto put_box = [&](const uint32_t (&w)[16], __nv_bfloat16* to, uint32_t row0, uint32_t col0) {
+      __syncwarp();  // every lane has read the previous box
 #pragma unroll
       for (uint32_t v = 0; v < 4; ++v) ptx::st_shared_v4(my_row + ((v ^ sw) * 16u), w[v * 4], w[v * 4 + 1], w[v * 4 + 2], w[v * 4 + 3]);
-      ptx::fence_proxy_async();
       __syncwarp();
-      if (lane == 0) {
-        // a box outside the result commits an empty group: the wait above counts groups
-        if (row0 < M && col0 < N) ptx::tma_store_2d(map, buf, static_cast<int32_t>(col0), static_cast<int32_t>(row0));
-        ptx::tma_store_commit();
-      }
+      const uint32_t col = col0 + tchunk * 8;
+      uint4* at = reinterpret_cast<uint4*>(to + static_cast<size_t>(row0 + trow) * N + col);
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)  // N % 8 == 0: a chunk is inside or outside as a whole
+        if (row0 + trow + 8 * i < M && col < N) at[static_cast<size_t>(i) * N] = ptx::ld_shared_u4(stage_box + turned(i));
     };
     auto pack = [](uint32_t lo, uint32_t hi) -> uint32_t {
       const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(lo), __uint_as_float(hi));
@@ -303,14 +310,25 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
         r[j + 3] = __float_as_uint(__uint_as_float(r[j + 3]) + q.w);
       }
     };
-    // The residual of one box: this lane's row, 32 columns.
-    auto load_residual = [&](uint4 (&q)[4], uint32_t row, uint32_t col0) {
+    // The residual of one box, turned like a result: whole 64-byte row segments from global memory, ...
+    auto load_residual = [&](uint4 (&q)[4], uint32_t row0, uint32_t col0) {
+      const uint32_t col = col0 + tchunk * 8;
+      const uint4* at = reinterpret_cast<const uint4*>(args.residual + static_cast<size_t>(row0 + trow) * N + col);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        q[v] = make_uint4(0u, 0u, 0u, 0u);
-        if (row < M && col0 + v * 8 < N)
-          q[v] = *reinterpret_cast<const uint4*>(args.residual + static_cast<size_t>(row) * N + col0 + v * 8);
+      for (uint32_t i = 0; i < 4; ++i) {
+        q[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row0 + trow + 8 * i < M && col < N) q[i] = at[static_cast<size_t>(i) * N];
       }
+    };
+    // ... and through the warp's second buffer to this lane's row of 32 columns.
+    auto turn_residual = [&](uint4 (&q)[4]) {
+      const uint32_t buf = kFfnStageBox;
+      __syncwarp();
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) ptx::st_shared_v4(stage_box + buf + turned(i), q[i].x, q[i].y, q[i].z, q[i].w);
+      __syncwarp();
+#pragma unroll
+      for (uint32_t v = 0; v < 4; ++v) q[v] = ptx::ld_shared_u4(my_row + buf + ((v ^ sw) * 16u));
     };
 
     for (uint32_t t = first; t < num_tiles; t += step, unit += NACC) {
@@ -350,109 +368,140 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
       };
       uint4 res[4];
       if (have_res) {
-        // this warp's share of the tile's residual on its way to L2 while the K loop runs: a lane's row is 2 KB and more
-        // from its neighbour's, so a load from HBM per box would be a full latency each (8192^3 with gelu, residual and
-        // stored projections: 1,170 -> see the launcher)
+        // this warp's share of the tile's residual on its way to L2 while the K loop runs
 #pragma unroll
         for (int a = 0; a < NACC; ++a) {
           const uint32_t row = row_t + a * 128 * CTAS + lane;
           if (row < M && out_col < N)
             ptx::prefetch_l2(args.residual + static_cast<size_t>(row) * N + out_col, min(static_cast<uint32_t>(TN / 2), N - out_col) * 2u);
         }
-        load_residual(res, row_t + lane, out_col);
+        load_residual(res, row_t, out_col);
       }
-      uint32_t r[NB][32];
+      // From accumulators to packed results: bias, the stored projections, activation, product or residual. `up` is r
+      // itself where there is no second projection. The next box's residual is under way afterwards.
+      auto finish = [&](uint32_t (&r)[32], uint32_t (&up)[32], uint32_t (&w)[16], int a, int q) {
+        const uint32_t row0 = row_t + a * 128 * CTAS, col0 = out_col + q * 32;
+        if constexpr (EPILOGUE) {
+          if (have_bias) {
+            add_bias(r, bias_s + half * (TN / 2) + q * 32);
+            if constexpr (GATED) add_bias(up, bias_s + TN + half * (TN / 2) + q * 32);
+          }
+          if (args.save) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = pack(r[2 * j], r[2 * j + 1]);
+            put_box(w, args.z[0], row0, col0);
+            if constexpr (GATED) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) w[j] = pack(up[2 * j], up[2 * j + 1]);
+              put_box(w, args.z[1], row0, col0);
+            }
+          }
+#pragma unroll
+          for (int j0 = 0; j0 < 32; j0 += 8) {
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(r[j0 + j]);
+            act_values<ACT>(f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              if constexpr (GATED) f[j] *= __uint_as_float(up[j0 + j]);
+              r[j0 + j] = __float_as_uint(f[j]);
+            }
+          }
+          if (have_res) {
+            turn_residual(res);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const uint32_t p[4] = {res[v].x, res[v].y, res[v].z, res[v].w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                r[v * 8 + 2 * j] = __float_as_uint(__uint_as_float(r[v * 8 + 2 * j]) + __uint_as_float(p[j] << 16));
+                r[v * 8 + 2 * j + 1] = __float_as_uint(__uint_as_float(r[v * 8 + 2 * j + 1]) + __uint_as_float(p[j] & 0xffff0000u));
+              }
+            }
+            if (q + 1 < OB) load_residual(res, row0, col0 + 32);
+            else if (a + 1 < NACC) load_residual(res, row0 + 128 * CTAS, out_col);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack(r[2 * j], r[2 * j + 1]);
+      };
       if (num_st > 0) {
         wait_acc(0);
         if (!ok) continue;
-        // the whole share of the first accumulator into registers: it is handed back before anything is computed
-#pragma unroll
-        for (int q = 0; q < NB; ++q) ptx::tmem_ld_32x32(acc_addr(0, q), r[q]);
-#pragma unroll
-        for (int q = 0; q < NB; ++q) ptx::tmem_ld_wait_for(r[q]);
-        release_acc(0);
-      } else {  // an empty contraction: the accumulators' initial value
-#pragma unroll
-        for (int q = 0; q < NB; ++q)
-#pragma unroll
-          for (int j = 0; j < 32; ++j) r[q][j] = 0u;
       }
+      if constexpr (NACC == 1) {
+        // One accumulator per tile and more in TMEM: there is no hurry to hand it back. The boxes go through one copy of
+        // the code: where a CTA has a single tile, fetching the instructions of four unrolled boxes for the first time
+        // took longer than running them (about 1,000 cycles each).
+#pragma unroll 1
+        for (int q = 0; q < OB; ++q) {
+          uint32_t r[32], up[GATED ? 32 : 1], w[16];
+          if (num_st > 0) {
+            ptx::tmem_ld_32x32(acc_addr(0, q), r);
+            if constexpr (GATED) {
+              ptx::tmem_ld_32x32(acc_addr(0, OB + q), up);
+              ptx::tmem_ld_wait_for(up);
+            }
+            ptx::tmem_ld_wait_for(r);
+            if (q + 1 == OB) release_acc(0);
+          } else {  // an empty contraction: the accumulators' initial value
 #pragma unroll
-      for (int a = 0; a < NACC; ++a) {
-        const uint32_t row0 = row_t + a * 128 * CTAS;
-        if (a > 0 && num_st > 0) {
+            for (int j = 0; j < 32; ++j) {
+              r[j] = 0u;
+              if constexpr (GATED) up[j] = 0u;
+            }
+          }
+          if constexpr (GATED) finish(r, up, w, 0, q);
+          else finish(r, r, w, 0, q);
+          put_box(w, args.c[which], row_t, out_col + q * 32);
+        }
+      } else {
+        uint32_t r[NB][32];
+        if (num_st > 0) {
+          // the whole share of the first accumulator into registers: it is handed back before anything is computed
+#pragma unroll
+          for (int q = 0; q < NB; ++q) ptx::tmem_ld_32x32(acc_addr(0, q), r[q]);
 #pragma unroll
           for (int q = 0; q < NB; ++q) ptx::tmem_ld_wait_for(r[q]);
-          release_acc(a);
+          release_acc(0);
+        } else {
+#pragma unroll
+          for (int q = 0; q < NB; ++q)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[q][j] = 0u;
         }
 #pragma unroll
-        for (int q = 0; q < OB; ++q) {
-          constexpr int up = GATED ? OB : 0;
-          const uint32_t col0 = out_col + q * 32;
-          uint32_t w[16];
-          if constexpr (EPILOGUE) {
-            if (have_bias) {
-              add_bias(r[q], bias_s + half * (TN / 2) + q * 32);
-              if constexpr (GATED) add_bias(r[up + q], bias_s + TN + half * (TN / 2) + q * 32);
-            }
-            if (args.save) {
+        for (int a = 0; a < NACC; ++a) {
+          if (a > 0 && num_st > 0) {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) w[j] = pack(r[q][2 * j], r[q][2 * j + 1]);
-              put_box(w, &args.z[0], row0, col0);
-              if constexpr (GATED) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) w[j] = pack(r[up + q][2 * j], r[up + q][2 * j + 1]);
-                put_box(w, &args.z[1], row0, col0);
-              }
-            }
-#pragma unroll
-            for (int j0 = 0; j0 < 32; j0 += 8) {
-              float f[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(r[q][j0 + j]);
-              act_values<ACT>(f);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                if constexpr (GATED) f[j] *= __uint_as_float(r[up + q][j0 + j]);
-                r[q][j0 + j] = __float_as_uint(f[j]);
-              }
-            }
-            if (have_res) {
-#pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                const uint32_t p[4] = {res[v].x, res[v].y, res[v].z, res[v].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  r[q][v * 8 + 2 * j] = __float_as_uint(__uint_as_float(r[q][v * 8 + 2 * j]) + __uint_as_float(p[j] << 16));
-                  r[q][v * 8 + 2 * j + 1] = __float_as_uint(__uint_as_float(r[q][v * 8 + 2 * j + 1]) + __uint_as_float(p[j] & 0xffff0000u));
-                }
-              }
-              // the next box's is under way while this one is stored
-              if (q + 1 < OB) load_residual(res, row0 + lane, col0 + 32);
-              else if (a + 1 < NACC) load_residual(res, row0 + 128 * CTAS + lane, out_col);
-            }
+            for (int q = 0; q < NB; ++q) ptx::tmem_ld_wait_for(r[q]);
+            release_acc(a);
           }
 #pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = pack(r[q][2 * j], r[q][2 * j + 1]);
-          if (a + 1 < NACC && num_st > 0) {  // this block's registers are free: refill them from the next accumulator
-            if (q == 0) wait_acc(a + 1);
-            if (ok) {
-              ptx::tmem_ld_32x32(acc_addr(a + 1, q), r[q]);
-              if constexpr (GATED) ptx::tmem_ld_32x32(acc_addr(a + 1, up + q), r[up + q]);
+          for (int q = 0; q < OB; ++q) {
+            constexpr int up = GATED ? OB : 0;
+            uint32_t w[16];
+            finish(r[q], r[up + q], w, a, q);
+            if (a + 1 < NACC && num_st > 0) {  // this block's registers are free: refill them from the next accumulator
+              if (q == 0) wait_acc(a + 1);
+              if (ok) {
+                ptx::tmem_ld_32x32(acc_addr(a + 1, q), r[q]);
+                if constexpr (GATED) ptx::tmem_ld_32x32(acc_addr(a + 1, up + q), r[up + q]);
+              }
             }
+            put_box(w, args.c[which], row_t + a * 128 * CTAS, out_col + q * 32);
           }
-          put_box(w, &args.c[which], row0, col0);
+          if (!ok) break;
         }
-        if (!ok) break;
       }
     }
-    if (lane == 0) ptx::tma_store_wait_all();  // every box has reached global memory before the CTA exits
   }
 
   ptx::tc_fence_before();
   __syncthreads();
   if (PAIR) {  // neither CTA may exit or free TMEM while the other can still signal it or read its shared memory
-    ptx::cluster_arrive();
+    ptx::cluster_arrive_relaxed();
     ptx::cluster_wait();
   }
   if (warp == 1) {

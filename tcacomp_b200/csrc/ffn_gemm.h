@@ -30,6 +30,18 @@ struct FfnProblem {
 int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t s);
 int ffn_device_status(int* out);
 
+// ffn_small.cuh: few rows or few output tiles
+struct FfnSmallPlan {
+  int tm = 128;                 // output rows per tile
+  uint64_t tiles = 0;
+  uint32_t ks = 1, blocks_per_range = 0;  // CTAs per tile (1, 2, 4, 8), K blocks of each
+  int per_sm = 1;                         // CTAs that share an SM
+  double us = 0;                          // the estimate that chose them
+};
+FfnSmallPlan ffn_small_plan(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sms, int forced_ks);
+int launch_ffn_small(const char* op, int form, const FfnProblem& p, cudaStream_t s);
+int ffn_small_status(int* out);
+
 // dz = dc * act'(z) (gated: dgate = dh * up * act'(gate), dup = dh * act(gate)), with the column sums of each where
 // wanted (act_backward.cu). dz may be null (column sums alone; act none). Partials of the sums go to `ws`.
 uint64_t act_backward_workspace(uint32_t rows, uint32_t cols, int gated);

@@ -197,6 +197,8 @@ ln_bwd_ring(const T* __restrict__ dy, const T* __restrict__ x, const T* __restri
     ptx::fence_proxy_async();
   }
   __syncthreads();
+  ptx::pdl_wait();
+  ptx::pdl_launch();
 
   auto issue = [&](uint64_t chunk, uint32_t s) {  // thread 0
     const uint64_t from = chunk * chunk_bytes, start = from & ~15ull, end = from + chunk_bytes < total ? from + chunk_bytes : total;
@@ -500,6 +502,8 @@ __global__ void __launch_bounds__(256)
 ln_bwd_finish(const float* __restrict__ partial, uint32_t parts, uint32_t cols, float* __restrict__ dgamma,
               float* __restrict__ dbeta) {
   __shared__ float sums[8][33];
+  ptx::pdl_wait();
+  ptx::pdl_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t c = static_cast<uint64_t>(blockIdx.x) * 32 + lane, width = 2ull * cols;
   float v = 0.0f;
@@ -600,8 +604,8 @@ int launch_ring(const Plan& p, const Call<T>& c) {
     cudaGetLastError();
     return fail(TCAB_ERR_CUDA, "layernorm_rows_backward: cannot reserve %u bytes of shared memory: %s", smem, cudaGetErrorString(e));
   }
-  fn<<<p.parts, p.groups * p.tpr, smem, c.s>>>(c.dy, c.x, c.gamma, c.mean, c.rstd, c.dx, c.part, c.rows, c.cols, p.tpr, p.groups,
-                                               p.stages, p.plane);
+  launch_pdl(fn, dim3(p.parts), dim3(p.groups * p.tpr), smem, c.s, c.dy, c.x, c.gamma, c.mean, c.rstd, c.dx, c.part, c.rows,
+             c.cols, p.tpr, p.groups, p.stages, p.plane);
   count_launch();
   return check_launch("ln_bwd_ring");
 }
@@ -671,7 +675,8 @@ int launch(const T* dy, const T* x, const T* gamma, const float* mean, const flo
     rc = launch_v<T, 1>(p, c);
   }
   if (rc != TCAB_OK || p.parts <= 1) return rc;
-  ln_bwd_finish<<<static_cast<unsigned>((2ull * cols + 31) / 32), 256, 0, s>>>(partial, p.parts, cols, dgamma, dbeta);
+  launch_pdl(ln_bwd_finish, dim3(static_cast<unsigned>((2ull * cols + 31) / 32)), dim3(256), 0, s,
+             static_cast<const float*>(partial), p.parts, cols, dgamma, dbeta);
   count_launch();
   return check_launch("ln_bwd_finish");
 }

@@ -28,10 +28,12 @@ def ints(*shape, seed, lo=-2, hi=3):
     return torch.randint(lo, hi, shape, device="cuda", generator=g).to(BF)
 
 
-@pytest.fixture(params=[0, 1, 2, 3], ids=["chosen", "512x256", "256x256", "128x128"])
+@pytest.fixture(params=[(0, 0), (1, 0), (2, 0), (3, 0), (4, 1), (4, 2), (4, 8)],
+                ids=["chosen", "512x256", "256x256", "128x128", "cluster1", "cluster2", "cluster8"])
 def tile(request, tcab_lib):
+    """Every kernel whatever the size: the tile shapes of the persistent one, and the one with a tile per cluster."""
     import tcacomp_b200 as T
-    T.tune("ffn", 0, request.param)
+    T.tune("ffn", 0, request.param[0], 0, request.param[1])
     yield request.param
     T.tune("ffn")
 
