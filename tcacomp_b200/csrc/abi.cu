@@ -83,6 +83,22 @@ int check_launch(const char* what) {
   return TCAB_OK;
 }
 
+// The attribute belongs to the device's copy of the function and stays set; the largest size asked for is remembered.
+int reserve_smem(const char* op, const void* fn, size_t bytes) {
+  static std::map<std::pair<int, const void*>, size_t> reserved;
+  const auto key = std::make_pair(current_device(), fn);
+  std::lock_guard<std::mutex> lk(g_mu);
+  size_t& have = reserved[key];
+  if (have >= bytes) return TCAB_OK;
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(TCAB_ERR_CUDA, "%s: cannot reserve %zu bytes of shared memory: %s", op, bytes, cudaGetErrorString(e));
+  }
+  have = bytes;
+  return TCAB_OK;
+}
+
 const Tune& tune(int family) { return g_tune[family]; }
 
 int occupancy(const void* fn, int block, size_t smem) {

@@ -28,6 +28,7 @@ void count_launch(unsigned n = 1);
 int sm_count();             // SMs of the current device (cached per device)
 int max_optin_smem();       // opt-in shared memory per block of the current device
 int check_launch(const char* what);  // cudaGetLastError -> status
+int reserve_smem(const char* op, const void* fn, size_t bytes);  // dynamic shared memory of a kernel, once per device and size
 
 struct Tune {
   int p0 = 0, p1 = 0, p2 = 0, p3 = 0;

@@ -128,11 +128,7 @@ int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t 
   }
   const FfnKernel k = kernel_of(form, p.act, shape);
   if (k.fn == nullptr) return fail(TCAB_ERR_UNSUPPORTED, "%s: no kernel for activation %d", op, p.act);
-  const cudaError_t ae = cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(k.smem));
-  if (ae != cudaSuccess) {
-    cudaGetLastError();
-    return fail(TCAB_ERR_CUDA, "%s: cannot reserve %zu bytes of shared memory: %s", op, k.smem, cudaGetErrorString(ae));
-  }
+  TCAB_TRY_RC(reserve_smem(op, k.fn, k.smem));
   const uint64_t tiles = static_cast<uint64_t>((p.M + bm - 1) / bm) * ((p.N + tile_n - 1) / tile_n) * (form == kFfnDw ? nb : 1);
   uint64_t groups = (tn.p0 > 0 ? static_cast<uint64_t>(tn.p0) : static_cast<uint64_t>(sm_count())) / ctas;
   if (groups > tiles) groups = tiles;

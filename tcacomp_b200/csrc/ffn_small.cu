@@ -95,11 +95,7 @@ int launch_ffn_small(const char* op, int form, const FfnProblem& p, cudaStream_t
       }
     }
   }
-  const cudaError_t ae = cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (ae != cudaSuccess) {
-    cudaGetLastError();
-    return fail(TCAB_ERR_CUDA, "%s: cannot reserve %zu bytes of shared memory: %s", op, smem, cudaGetErrorString(ae));
-  }
+  TCAB_TRY_RC(reserve_smem(op, k.fn, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(plan.tiles * plan.ks));
   cfg.blockDim = dim3(kSmallThreads);

@@ -599,11 +599,7 @@ int launch_ring(const Plan& p, const Call<T>& c) {
   uint32_t smem = 2 * p.plane * p.stages;
   const uint32_t sums = p.groups * c.cols * 4;  // the groups' column sums at the end
   if (smem < sums) smem = sums;
-  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return fail(TCAB_ERR_CUDA, "layernorm_rows_backward: cannot reserve %u bytes of shared memory: %s", smem, cudaGetErrorString(e));
-  }
+  TCAB_TRY_RC(reserve_smem("layernorm_rows_backward", reinterpret_cast<const void*>(fn), smem));
   launch_pdl(fn, dim3(p.parts), dim3(p.groups * p.tpr), smem, c.s, c.dy, c.x, c.gamma, c.mean, c.rstd, c.dx, c.part, c.rows,
              c.cols, p.tpr, p.groups, p.stages, p.plane);
   count_launch();
