@@ -7,34 +7,18 @@
 #ifdef __CUDACC__
 namespace tcab {
 
-using f32x2 = uint64_t;
+using f32x2 = float2;
 
-__device__ __forceinline__ f32x2 pair_of(float lo, float hi) {
-  f32x2 p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
-  return p;
+__device__ __forceinline__ f32x2 pair_of(float lo, float hi) { return make_float2(lo, hi); }
+__device__ __forceinline__ void pair_to(f32x2 p, float& lo, float& hi) {
+  lo = p.x;
+  hi = p.y;
 }
-__device__ __forceinline__ void pair_to(f32x2 p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
-__device__ __forceinline__ float pair_sum(f32x2 p) {
-  float lo, hi;
-  pair_to(p, lo, hi);
-  return lo + hi;
-}
-__device__ __forceinline__ f32x2 fma_pair(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ f32x2 mul_pair(f32x2 a, f32x2 b) {
-  f32x2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ f32x2 add_pair(f32x2 a, f32x2 b) {
-  f32x2 d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
+__device__ __forceinline__ float pair_sum(f32x2 p) { return p.x + p.y; }
+__device__ __forceinline__ f32x2 fma_pair(f32x2 a, f32x2 b, f32x2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ f32x2 mul_pair(f32x2 a, f32x2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ f32x2 add_pair(f32x2 a, f32x2 b) { return __fadd2_rn(a, b); }
+
 // the same operations on one value, for kernels that handle both
 __device__ __forceinline__ float fma_pair(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ float mul_pair(float a, float b) { return a * b; }

@@ -28,7 +28,7 @@ int ffn_small_status(int* out) {
 // launches (contractions over 64 to 4096, outputs of 4096 columns):
 //   before the first and behind the last block: 3.2 (16 or 32 rows), 4.3 (64), 5.8 (128); + 0.1, 0.2, 1.1 (6 from 64 rows on)
 //   for 2, 4, 8 ranges
-//   a block of 64: 0.33, or the time HBM takes for the blocks of all ranges (5.2 TB/s)
+//   a block of 64: 0.33, or the time HBM takes for the blocks of all ranges (6.3 TB/s from two CTAs per SM, 4.6 from one)
 // 1 x 4096 x 4096: 22.3, 14.6, 11.7, 9.5 us for 1, 2, 4, 8 ranges; 128 rows: 27.6, 17.1, 12.8, 26.6.
 FfnSmallPlan ffn_small_plan(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sms, int forced_ks) {
   FfnSmallPlan p;
@@ -45,7 +45,7 @@ FfnSmallPlan ffn_small_plan(int form, uint32_t m, uint32_t n, uint32_t k, uint32
     const int per_sm = p.tm < 128 && ctas > static_cast<uint64_t>(sms) ? 2 : 1;
     const uint64_t slots = static_cast<uint64_t>(sms) * per_sm, rounds = (ctas + slots - 1) / slots;
     const double resident = static_cast<double>(ctas < slots ? ctas : slots) / static_cast<double>(p.tiles);
-    double block = static_cast<double>(wide) * resident * 16384.0 / 5.2e6;
+    double block = static_cast<double>(wide) * resident * 16384.0 / (per_sm == 2 ? 6.3e6 : 4.6e6);
     if (block < 0.33) block = 0.33;
     const double ranges = ks == 1 ? 0.0 : ks == 2 ? 0.1 : ks == 4 ? 0.2 : p.tm <= 32 ? 1.1 : 6.0;
     const double us = (p.tm <= 32 ? 3.2 : p.tm == 64 ? 4.3 : 5.8) * (0.5 + 0.5 * static_cast<double>(rounds)) + ranges +

@@ -97,7 +97,7 @@ ffn_small_kernel(const __grid_constant__ FfnSmallArgs args) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_p = &abort_flag;
   const uint32_t M = args.M, N = args.N, ks = args.ks, stages = args.stages;
-  const uint32_t receive = ring + stages * C::STAGE;
+  const uint32_t receive = ring + stages * C::STAGE, first_blocks = min(stages, 3u);
   const uint32_t rank = ks > 1 ? ptx::cluster_ctarank() : 0u;  // the range; clusters are ks x 1 x 1 over a 1-D grid
   const uint32_t tiles_m = (M + TM - 1) / TM, tiles_n = (N + TN - 1) / TN, tiles_one = tiles_m * tiles_n;
   uint32_t tile = blockIdx.x / ks;
@@ -142,8 +142,9 @@ ffn_small_kernel(const __grid_constant__ FfnSmallArgs args) {
     ptx::fence_barrier_init();
     ptx::fence_proxy_async();
     ptx::pdl_wait();
-    // the first blocks are under way before the TMEM allocation and the barrier below
-    for (uint32_t i = 0; i < num_kb && i < stages; ++i) issue(i, i);
+    // the first blocks are under way before the TMEM allocation and the barrier below; the others follow it: a full ring
+    // of copies from one thread takes 1,500 cycles
+    for (uint32_t i = 0; i < num_kb && i < first_blocks; ++i) issue(i, i);
   }
   __syncwarp();
   if (ks > 1) ptx::cluster_arrive();  // this CTA's barriers are initialised
@@ -159,6 +160,7 @@ ffn_small_kernel(const __grid_constant__ FfnSmallArgs args) {
 
   if (warp == 0) {
     if (lane == 0) {
+      for (uint32_t i = first_blocks; i < stages && i < num_kb; ++i) issue(i, i);
       uint32_t stage = 0, phase = 0;
       for (uint32_t i = stages; i < num_kb; ++i) {
         if (!ptx::mbar_wait(ptx::smem_u32(&bar_empty[stage]), phase, abort_p)) break;

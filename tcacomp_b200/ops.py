@@ -443,9 +443,10 @@ _empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", N
 
 
 def _new(shape: tuple, dtype: torch.dtype) -> torch.Tensor:
-    if _empty_strided is None or len(shape) > 2:
+    rank = len(shape)
+    if _empty_strided is None or rank > 2:
         return torch.empty(shape, device="cuda", dtype=dtype)
-    return _empty_strided(shape, (1,) if len(shape) == 1 else (shape[1], 1), dtype)
+    return _empty_strided(shape, (1,) if rank == 1 else (shape[1], 1), dtype)
 
 
 def _packed_new(t: torch.Tensor, name: str, dev: int) -> bytes:
@@ -514,7 +515,7 @@ def layernorm_rows_stats(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tenso
         xv = _packed(x, "x", dev)
         yp = mp = rp = _packed
         if out is None:
-            out, yp = torch.empty_like(x), _packed_new
+            out, yp = _new(x.shape, x.dtype), _packed_new
         if mean is None:
             mean, mp = _new(tuple(x.shape[:-1]) or (1,), torch.float32), _packed_new
         if rstd is None:
@@ -537,7 +538,7 @@ def layernorm_rows_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tens
         xv = _packed(x, "x", dev)
         xp = gp = bp = _packed
         if dx is None:
-            dx, xp = torch.empty_like(x), _packed_new
+            dx, xp = _new(x.shape, x.dtype), _packed_new
         if dgamma is None:
             dgamma, gp = _new((x.shape[-1],), torch.float32), _packed_new
         if dbeta is None:
