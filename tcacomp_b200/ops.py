@@ -515,7 +515,7 @@ def layernorm_rows_stats(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tenso
         xv = _packed(x, "x", dev)
         yp = mp = rp = _packed
         if out is None:
-            out, yp = _new(x.shape, x.dtype), _packed_new
+            out, yp = _new(tuple(x.shape), x.dtype), _packed_new
         if mean is None:
             mean, mp = _new(tuple(x.shape[:-1]) or (1,), torch.float32), _packed_new
         if rstd is None:
@@ -538,7 +538,7 @@ def layernorm_rows_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tens
         xv = _packed(x, "x", dev)
         xp = gp = bp = _packed
         if dx is None:
-            dx, xp = _new(x.shape, x.dtype), _packed_new
+            dx, xp = _new(tuple(x.shape), x.dtype), _packed_new
         if dgamma is None:
             dgamma, gp = _new((x.shape[-1],), torch.float32), _packed_new
         if dbeta is None:
