@@ -180,6 +180,109 @@ func GemmBiasAct(a, b Tensor, bias *Tensor, relu bool, c Tensor, stream unsafe.P
 	return call(func() C.int { return C.tcab_gemm_bias_act(&ca, &cb, pb, act, &cc, stream) })
 }
 
+// Act names an epilogue activation of the feed-forward operators (tcab_act).
+type Act C.int
+
+const (
+	ActNone     = Act(C.TCAB_ACT_NONE)
+	ActRelu     = Act(C.TCAB_ACT_RELU)
+	ActSilu     = Act(C.TCAB_ACT_SILU)
+	ActGelu     = Act(C.TCAB_ACT_GELU)
+	ActGeluTanh = Act(C.TCAB_ACT_GELU_TANH)
+	ActSigmoid  = Act(C.TCAB_ACT_SIGMOID) // the gated forms only
+)
+
+// opt is the C view of an optional tensor.
+func opt(p *Tensor) *C.tcab_tensor {
+	if p == nil {
+		return nil
+	}
+	v := p.c()
+	return &v
+}
+
+// LayernormRowsStats is LayernormRows that also stores each row's mean and
+// 1 / sqrt(var + eps) for LayernormRowsBackward. tcab_layernorm_rows_stats.
+func LayernormRowsStats(x, gamma, beta Tensor, eps float32, y, mean, rstd Tensor, stream unsafe.Pointer) error {
+	cx, cg, cb, cy, cm, cr := x.c(), gamma.c(), beta.c(), y.c(), mean.c(), rstd.c()
+	return call(func() C.int {
+		return C.tcab_layernorm_rows_stats(&cx, &cg, &cb, C.float(eps), &cy, &cm, &cr, stream)
+	})
+}
+
+// LayernormRowsBackwardWorkspace is the bytes of device memory LayernormRowsBackward needs for rows like x.
+func LayernormRowsBackwardWorkspace(x Tensor) uint64 {
+	cx := x.c()
+	return uint64(C.tcab_layernorm_rows_backward_workspace(&cx))
+}
+
+// LayernormRowsBackward computes dx, dgamma and dbeta. tcab_layernorm_rows_backward.
+func LayernormRowsBackward(dy, x, gamma, mean, rstd, dx, dgamma, dbeta Tensor, workspace unsafe.Pointer,
+	workspaceBytes uint64, stream unsafe.Pointer) error {
+	cdy, cx, cg, cm, cr, cdx, cdg, cdb := dy.c(), x.c(), gamma.c(), mean.c(), rstd.c(), dx.c(), dgamma.c(), dbeta.c()
+	return call(func() C.int {
+		return C.tcab_layernorm_rows_backward(&cdy, &cx, &cg, &cm, &cr, &cdx, &cdg, &cdb, workspace,
+			C.uint64_t(workspaceBytes), stream)
+	})
+}
+
+// GemmBiasActResidual launches c = act(a @ b + bias) + residual; preact, where
+// given, receives a @ b + bias. tcab_gemm_bias_act_residual.
+func GemmBiasActResidual(a, b Tensor, bias, residual *Tensor, act Act, preact *Tensor, c Tensor, stream unsafe.Pointer) error {
+	ca, cb, cbias, cres, cpre, cc := a.c(), b.c(), opt(bias), opt(residual), opt(preact), c.c()
+	return call(func() C.int {
+		return C.tcab_gemm_bias_act_residual(&ca, &cb, cbias, cres, C.int(act), cpre, &cc, stream)
+	})
+}
+
+// GemmBiasActBackwardWorkspace is the bytes of device memory GemmBiasActBackward needs.
+func GemmBiasActBackwardWorkspace(m, n uint32, act Act, withDbias bool) uint64 {
+	return uint64(C.tcab_gemm_bias_act_backward_workspace(C.uint32_t(m), C.uint32_t(n), C.int(act), flag(withDbias)))
+}
+
+// GemmBiasActBackward computes those of da, db and dbias that are given. tcab_gemm_bias_act_backward.
+func GemmBiasActBackward(dc, a, b Tensor, preact *Tensor, act Act, da, db, dbias *Tensor, workspace unsafe.Pointer,
+	workspaceBytes uint64, stream unsafe.Pointer) error {
+	cdc, ca, cb, cpre, cda, cdb, cdbias := dc.c(), a.c(), b.c(), opt(preact), opt(da), opt(db), opt(dbias)
+	return call(func() C.int {
+		return C.tcab_gemm_bias_act_backward(&cdc, &ca, &cb, cpre, C.int(act), cda, cdb, cdbias, workspace,
+			C.uint64_t(workspaceBytes), stream)
+	})
+}
+
+// GatedGemm launches h = act(x @ wGate + biasGate) * (x @ wUp + biasUp); gate
+// and up, where given, receive the two projections. tcab_gated_gemm.
+func GatedGemm(x, wGate, wUp Tensor, biasGate, biasUp *Tensor, act Act, gate, up *Tensor, h Tensor, stream unsafe.Pointer) error {
+	cx, cg, cu, cbg, cbu, cgate, cup, ch := x.c(), wGate.c(), wUp.c(), opt(biasGate), opt(biasUp), opt(gate), opt(up), h.c()
+	return call(func() C.int {
+		return C.tcab_gated_gemm(&cx, &cg, &cu, cbg, cbu, C.int(act), cgate, cup, &ch, stream)
+	})
+}
+
+// GatedGemmBackwardWorkspace is the bytes of device memory GatedGemmBackward needs.
+func GatedGemmBackwardWorkspace(m, n uint32, withDbias bool) uint64 {
+	return uint64(C.tcab_gated_gemm_backward_workspace(C.uint32_t(m), C.uint32_t(n), flag(withDbias)))
+}
+
+// GatedGemmBackward computes those gradients that are given (the weights' both
+// or neither, the biases' likewise). tcab_gated_gemm_backward.
+func GatedGemmBackward(dh, x, wGate, wUp, gate, up Tensor, act Act, dx, dwGate, dwUp, dbiasGate, dbiasUp *Tensor,
+	workspace unsafe.Pointer, workspaceBytes uint64, stream unsafe.Pointer) error {
+	cdh, cx, cg, cu, cgate, cup := dh.c(), x.c(), wGate.c(), wUp.c(), gate.c(), up.c()
+	cdx, cdg, cdu, cbg, cbu := opt(dx), opt(dwGate), opt(dwUp), opt(dbiasGate), opt(dbiasUp)
+	return call(func() C.int {
+		return C.tcab_gated_gemm_backward(&cdh, &cx, &cg, &cu, &cgate, &cup, C.int(act), cdx, cdg, cdu, cbg, cbu,
+			workspace, C.uint64_t(workspaceBytes), stream)
+	})
+}
+
+func flag(b bool) C.int {
+	if b {
+		return 1
+	}
+	return 0
+}
+
 // Prepare compiles now what the first launch of a chain without an
 // ahead-of-time kernel would compile later (tcab_chain_prepare); use is one of
 // C.TCAB_USE_REDUCE, _CONTRACT, _MAP, _REDUCE_BATCHED. Not during a stream capture.
