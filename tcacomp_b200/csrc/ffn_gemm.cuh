@@ -107,47 +107,6 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
   const uint32_t num_st = FORM == kFfnDx ? seg_st * args.pairs : seg_st;
   const uint32_t first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
-  // The boxes of one ring stage: f(offset in the stage, tensor map, x, y) for each.
-  auto copies = [&](uint32_t t, uint32_t st, auto&& f) {
-    const uint32_t which = FORM == kFfnDw && t >= tiles_one ? 1u : 0u;
-    const FfnCoord tc = ffn_coord(t - which * tiles_one, tiles_m, tiles_n1);
-    const int32_t m0 = static_cast<int32_t>(tc.m * C::BM + rank * 128);  // accumulator a: + a * 128 CTAS
-    // Gated: a pair's first CTA loads the gate's columns, its second the same columns of up
-    const int32_t n0 = static_cast<int32_t>(tc.n * TN + (GATED ? 0u : rank * C::B_COLS));
-    const uint32_t seg = FORM == kFfnDx && st >= seg_st ? 1u : 0u;
-#pragma unroll
-    for (int kk = 0; kk < KPS; ++kk) {
-      const uint32_t a_at = kk * C::BLOCK, b_at = a_at + C::A_BYTES;
-      const int32_t k0 = static_cast<int32_t>(((st - seg * seg_st) * KPS + kk) * kFfnBK);
-#pragma unroll
-      for (int a = 0; a < NACC; ++a) {
-        const int32_t row = m0 + a * 128 * CTAS;
-        if (A_MN) {
-          f(a_at + a * 2 * kFfnAtom, &args.a[0], row, k0);
-          f(a_at + a * 2 * kFfnAtom + kFfnAtom, &args.a[0], row + 64, k0);
-        } else {
-          f(a_at + a * 2 * kFfnAtom, &args.a[seg], k0, row);
-        }
-      }
-      if (B_NK) {
-        f(b_at, &args.b[seg], k0, n0);
-      } else {
-#pragma unroll
-        for (int j = 0; j < C::B_COLS / 64; ++j) {
-          constexpr int per = GATED && !PAIR ? BN / 128 : 64;  // Gated on one CTA: boxes of gate, then of up
-          const uint32_t side = GATED ? (PAIR ? rank : static_cast<uint32_t>(j / per)) : which;
-          f(b_at + j * kFfnAtom, &args.b[side], n0 + (j % per) * 64, k0);
-        }
-      }
-    }
-  };
-
-  if (warp == 2 && lane == 0) {
-    // While barriers are set up (and, for a programmatic launch, the previous kernel drains) the first stages come to L2,
-    // the point where all SMs' writes meet: a prefetch returns nothing, so it cannot observe what a kernel still has to write.
-    for (uint32_t st = 0; st < num_st && st < C::STAGES; ++st)
-      copies(first, st, [&](uint32_t, const CUtensorMap* map, int32_t x, int32_t y) { ptx::tma_prefetch_2d(map, x, y); });
-  }
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < C::STAGES; ++s) {
@@ -183,25 +142,54 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
   ptx::pdl_wait();
   ptx::pdl_launch();
 
-  bool arrived = false;  // PAIR: at the cluster barrier that ends the kernel
   // Register split: 384 threads x 168 at launch = 64,512; 128 x 40 + 256 x 224 = 62,464 afterwards.
   if (warp < 4) {
     ptx::setmaxnreg_dec<40>();
     if (warp == 0) {
       // ---------------- TMA producer (every CTA) ----------------
       if (lane == 0) {
+        auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y) {
+          if (PAIR) ptx::tma_load_2d_pair(dst, map, bar, x, y);
+          else ptx::tma_load_2d(dst, map, bar, x, y);
+        };
         uint32_t stage = 0, phase = 0;
         bool ok = true;
         for (uint32_t t = first; ok && t < num_tiles; t += step) {
+          const uint32_t which = FORM == kFfnDw && t >= tiles_one ? 1u : 0u;
+          const FfnCoord tc = ffn_coord(t - which * tiles_one, tiles_m, tiles_n1);
+          const int32_t m0 = static_cast<int32_t>(tc.m * C::BM + rank * 128);  // accumulator a: + a * 128 CTAS
+          // Gated: a pair's first CTA loads the gate's columns, its second the same columns of up
+          const int32_t n0 = static_cast<int32_t>(tc.n * TN + (GATED ? 0u : rank * C::B_COLS));
           for (uint32_t st = 0; st < num_st; ++st) {
             if (!ptx::mbar_wait_parked(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, abort_p)) { ok = false; break; }
             const uint32_t full = PAIR ? ptx::mapa(ptx::smem_u32(&bar_full[stage]), 0) : ptx::smem_u32(&bar_full[stage]);
+            const uint32_t seg = FORM == kFfnDx && st >= seg_st ? 1u : 0u;
             if (leader) ptx::mbar_expect_tx(ptx::smem_u32(&bar_full[stage]), CTAS * C::STAGE);
-            copies(t, st, [&](uint32_t offset, const CUtensorMap* map, int32_t x, int32_t y) {
-              const uint32_t dst = smem_base + stage * C::STAGE + offset;
-              if (PAIR) ptx::tma_load_2d_pair(dst, map, full, x, y);
-              else ptx::tma_load_2d(dst, map, full, x, y);
-            });
+#pragma unroll
+            for (int kk = 0; kk < KPS; ++kk) {
+              const uint32_t a_dst = smem_base + stage * C::STAGE + kk * C::BLOCK, b_dst = a_dst + C::A_BYTES;
+              const int32_t k0 = static_cast<int32_t>(((st - seg * seg_st) * KPS + kk) * kFfnBK);
+#pragma unroll
+              for (int a = 0; a < NACC; ++a) {
+                const int32_t row = m0 + a * 128 * CTAS;
+                if (A_MN) {
+                  load(a_dst + a * 2 * kFfnAtom, &args.a[0], full, row, k0);
+                  load(a_dst + a * 2 * kFfnAtom + kFfnAtom, &args.a[0], full, row + 64, k0);
+                } else {
+                  load(a_dst + a * 2 * kFfnAtom, &args.a[seg], full, k0, row);
+                }
+              }
+              if (B_NK) {
+                load(b_dst, &args.b[seg], full, k0, n0);
+              } else {
+#pragma unroll
+                for (int j = 0; j < C::B_COLS / 64; ++j) {
+                  constexpr int per = GATED && !PAIR ? BN / 128 : 64;  // Gated on one CTA: boxes of gate, then of up
+                  const uint32_t side = GATED ? (PAIR ? rank : static_cast<uint32_t>(j / per)) : which;
+                  load(b_dst + j * kFfnAtom, &args.b[side], full, n0 + (j % per) * 64, k0);
+                }
+              }
+            }
             if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
           }
         }
@@ -372,18 +360,11 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
       };
       auto release_acc = [&](int a) {
         ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
+        // A signal that no later tile waits for is not sent: nothing of this CTA may be under way to a peer that has left.
+        if (lane == 0 && t + step * (C::SLOTS / NACC) < num_tiles) {
           const uint32_t bar = ptx::smem_u32(&bar_acc_empty[(unit + a) % C::SLOTS]);
           if (PAIR) ptx::mbar_arrive_cluster(ptx::mapa(bar, 0));
           else ptx::mbar_arrive(bar);
-        }
-        if (PAIR && a == NACC - 1 && t + step >= num_tiles) {
-          // The last that this warp signals to the peer: it meets the end of the pair here, before its last stores, so
-          // that the release does not wait for them.
-          __syncwarp();
-          ptx::cluster_arrive();
-          arrived = true;
         }
       };
       uint4 res[4];
@@ -521,7 +502,7 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
   ptx::tc_fence_before();
   __syncthreads();
   if (PAIR) {  // neither CTA may exit or free TMEM while the other can still signal it or read its shared memory
-    if (!arrived) ptx::cluster_arrive();
+    ptx::cluster_arrive_relaxed();
     ptx::cluster_wait();
   }
   if (warp == 1) {

@@ -151,13 +151,6 @@ __device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
-// The same tile on its way to L2; nothing waits for it.
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* m, int32_t x, int32_t y) {
-  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];"
-               ::"l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y)
-               : "memory");
-}
-
 // 2-D tiled store from this CTA's shared memory (bulk-group completion). Elements outside the
 // tensor are clipped by the hardware. x follows the same 16-byte rule as for loads and must not be
 // negative.
