@@ -89,6 +89,19 @@ TCAB_API int tcab_plan_row_shape(int op, int elem_bytes, uint32_t nvec, uint32_t
 TCAB_API int tcab_compile_check(const tcab_chain* chain, const int32_t* in_dtypes, uint32_t n_ins, int use,
                                 int out_dtype, int row_value_mask, int shared_row_mask, int cell_value_mask);
 
+/* The kernel a contraction of the feed-forward operators takes on a device of `sms` SMs. form: 0 forward, 1 gated, 2 the
+ * gradient of the left operand (contracts n of the forward pass; m, n, k are those of THIS contraction), 3 the gradient of
+ * the right one; pairs: operand pairs (2) or outputs (3). Outputs: rows and columns of a tile, CTAs that share a tile's
+ * contracted axis, and the blocks of 64 each of them takes. */
+TCAB_API int tcab_plan_ffn(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sms, uint32_t* rows, uint32_t* cols,
+                           uint32_t* ranges, uint32_t* blocks);
+
+/* How tcab_layernorm_rows_backward cuts up rows x cols elements (`aligned`: dy and x start on 16-byte boundaries):
+ * out[0] 0 = chunks through a shared-memory ring, 1 = two passes; then for the ring values per thread, threads per row,
+ * rows side by side per CTA, rows each of those takes at once, stages, bytes of a stage's half; out[7] = CTAs that leave
+ * partial column sums. */
+TCAB_API int tcab_plan_layernorm_backward(uint64_t rows, uint32_t cols, int elem_bytes, int aligned, int sms, uint32_t* out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -121,6 +121,9 @@ TUNING_SYMBOLS = [
     ("tcab_plan_outer_flat_ranges", C.c_int,
      [C.c_uint64, C.c_uint32, C.c_uint32, C.c_int, C.c_uint64, C.POINTER(C.c_uint32), C.POINTER(C.c_uint32),
       C.POINTER(C.c_uint32)]),
+    ("tcab_plan_ffn", C.c_int, [C.c_int] + [C.c_uint32] * 4 + [C.c_int] + [C.POINTER(C.c_uint32)] * 4),
+    ("tcab_plan_layernorm_backward", C.c_int,
+     [C.c_uint64, C.c_uint32, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_uint32)]),
     ("tcab_plan_outer_split", C.c_int,
      [C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint64, C.c_int, C.c_int, C.POINTER(C.c_uint32), C.POINTER(C.c_uint32)]),
 ]

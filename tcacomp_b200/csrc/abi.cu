@@ -510,6 +510,23 @@ int tcab_plan_outer_flat_ranges(uint64_t batches, uint32_t nk, uint32_t nc, int 
   return TCAB_OK;
 }
 
+int tcab_plan_ffn(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sms, uint32_t* rows, uint32_t* cols, uint32_t* ranges,
+                  uint32_t* blocks) {
+  if (rows == nullptr || cols == nullptr || ranges == nullptr || blocks == nullptr) return fail(TCAB_ERR_INVALID_ARG, "plan_ffn: null output");
+  if (form < kFfnFwd || form > kFfnDw || pairs < 1 || pairs > 2 || sms < 1)
+    return fail(TCAB_ERR_INVALID_ARG, "plan_ffn: form 0..3, one or two pairs, a positive SM count");
+  ffn_plan(form, m, n, k, pairs, sms, rows, cols, ranges, blocks);
+  return TCAB_OK;
+}
+
+int tcab_plan_layernorm_backward(uint64_t rows, uint32_t cols, int elem_bytes, int aligned, int sms, uint32_t* out) {
+  if (out == nullptr) return fail(TCAB_ERR_INVALID_ARG, "plan_layernorm_backward: null output");
+  if (cols < 1 || sms < 1 || (elem_bytes != 2 && elem_bytes != 4))
+    return fail(TCAB_ERR_INVALID_ARG, "plan_layernorm_backward: positive cols and sms, elements of 2 or 4 bytes");
+  layernorm_backward_plan(rows, cols, elem_bytes, aligned, sms, out);
+  return TCAB_OK;
+}
+
 int tcab_softmax_rows(const tcab_tensor* x, const tcab_tensor* y, void* stream) {
   const char* op = "softmax_rows";
   TCAB_TRY(check_tensor(op, "x", x));

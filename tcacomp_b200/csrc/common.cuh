@@ -93,6 +93,7 @@ int launch_layernorm_rows_f32(const float* x, const float* gamma, const float* b
 // layernorm_backward.cu; the workspace of a size covers every alignment of its operands
 uint64_t layernorm_backward_workspace(uint64_t rows, uint32_t cols, int elem_bytes);
 int layernorm_backward_status(int* out);
+void layernorm_backward_plan(uint64_t rows, uint32_t cols, int elem_bytes, int aligned, int sms, uint32_t* out);
 int launch_layernorm_backward_bf16(const __nv_bfloat16* dy, const __nv_bfloat16* x, const __nv_bfloat16* gamma, const float* mean,
                                    const float* rstd, __nv_bfloat16* dx, float* dgamma, float* dbeta, uint64_t rows, uint32_t cols,
                                    void* ws, uint64_t ws_bytes, cudaStream_t s);

@@ -50,16 +50,15 @@ constexpr int kShapes = 3, kCtas[kShapes] = {2, 2, 1}, kRows[kShapes] = {512, 25
 //   512 x 256 on pairs 8.3 + 0.49 per block, 256 x 256 on pairs 5.8 + 0.30, 128 x 128 3.6 + 0.30 (its two operand tiles per
 //   128 x 128 products are at the shared-memory limit), against 3.1-3.7 for a library product's launch.
 // Over many rounds the 512 x 256 tile wins (8192^3: 1,395 TFLOP/s against 1,305 for 256 x 256): it moves the fewest bytes.
-int choose(int form, const FfnProblem& p) {
+int choose(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sm) {
   static const double kFixed[kShapes] = {8.3, 5.8, 3.6}, kBlock[kShapes] = {0.49, 0.30, 0.30}, kEpilogue[kShapes] = {4.0, 2.2, 1.0};
-  const uint64_t sms = static_cast<uint64_t>(sm_count());
-  const uint32_t pairs = p.b[1] != nullptr ? 2 : 1;
-  const uint64_t outs = form == kFfnDw ? pairs : 1, blocks = (static_cast<uint64_t>(p.K) + 63) / 64 * (form == kFfnDx ? pairs : 1);
+  const uint64_t sms = static_cast<uint64_t>(sm);
+  const uint64_t outs = form == kFfnDw ? pairs : 1, blocks = (static_cast<uint64_t>(k) + 63) / 64 * (form == kFfnDx ? pairs : 1);
   int best = kShapes;
-  double best_us = ffn_small_plan(form, p.M, p.N, p.K, pairs, sm_count(), 0).us;
+  double best_us = ffn_small_plan(form, m, n, k, pairs, sm, 0).us;
   for (int s = 0; s < kShapes; ++s) {
     const uint64_t bm = kRows[s], tn = static_cast<uint64_t>(form == kFfnGated ? kBN[s] / 2 : kBN[s]);
-    const uint64_t tiles = (p.M + bm - 1) / bm * ((p.N + tn - 1) / tn) * outs, at_once = sms / kCtas[s];
+    const uint64_t tiles = (m + bm - 1) / bm * ((n + tn - 1) / tn) * outs, at_once = sms / kCtas[s];
     if (at_once == 0) continue;
     const uint64_t rounds = (tiles + at_once - 1) / at_once;
     // a round's end is hidden where two accumulators alternate; the 512 x 256 tile pays part of it every time
@@ -75,6 +74,25 @@ int choose(int form, const FfnProblem& p) {
 }
 
 }  // namespace
+
+// Rows and columns of a tile of the kernel that a contraction takes, the CTAs that share a tile's contracted axis and the
+// K blocks of 64 that each of them takes (ffn_small.cuh: columns are 128, of a gated pair 64 each).
+void ffn_plan(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sms, uint32_t* rows, uint32_t* cols, uint32_t* ranges,
+              uint32_t* blocks) {
+  const int shape = choose(form, m, n, k, pairs, sms);
+  if (shape == kShapes) {
+    const FfnSmallPlan p = ffn_small_plan(form, m, n, k, pairs, sms, 0);
+    *rows = static_cast<uint32_t>(p.tm);
+    *cols = form == kFfnGated ? 64 : 128;
+    *ranges = p.ks;
+    *blocks = p.blocks_per_range;
+    return;
+  }
+  *rows = static_cast<uint32_t>(kRows[shape]);
+  *cols = static_cast<uint32_t>(form == kFfnGated ? kBN[shape] / 2 : kBN[shape]);
+  *ranges = 1;
+  *blocks = static_cast<uint32_t>((static_cast<uint64_t>(k) + 63) / 64 * (form == kFfnDx ? pairs : 1));
+}
 
 int ffn_device_status(int* out) {
   *out = 0;
@@ -97,7 +115,7 @@ int ffn_device_status(int* out) {
 int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t s) {
   if (p.M == 0 || p.N == 0) return TCAB_OK;
   const Tune& tn = tune(kFfn);
-  const int shape = tn.p1 > 0 && tn.p1 <= kShapes + 1 ? tn.p1 - 1 : choose(form, p);
+  const int shape = tn.p1 > 0 && tn.p1 <= kShapes + 1 ? tn.p1 - 1 : choose(form, p.M, p.N, p.K, p.b[1] != nullptr ? 2 : 1, sm_count());
   if (shape == kShapes) return launch_ffn_small(op, form, p, s);
   const uint32_t ctas = kCtas[shape], bm = kRows[shape], bn = kBN[shape], tile_n = form == kFfnGated ? bn / 2 : bn;
   FfnArgs args = {};

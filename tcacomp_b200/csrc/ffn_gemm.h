@@ -41,6 +41,8 @@ struct FfnSmallPlan {
 FfnSmallPlan ffn_small_plan(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sms, int forced_ks);
 int launch_ffn_small(const char* op, int form, const FfnProblem& p, cudaStream_t s);
 int ffn_small_status(int* out);
+void ffn_plan(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sms, uint32_t* rows, uint32_t* cols, uint32_t* ranges,
+              uint32_t* blocks);
 
 // dz = dc * act'(z) (gated: dgate = dh * up * act'(gate), dup = dh * act(gate)), with the column sums of each where
 // wanted (act_backward.cu). dz may be null (column sums alone; act none). Partials of the sums go to `ws`.

@@ -536,9 +536,9 @@ struct Plan {
 // TB/s; four 3.4). With 16 values a second row would have to read its first half again (8192 columns: 5.2 -> 4.7).
 constexpr int ring_rows(int es, int values) { return es == 2 && values == 8 ? 2 : 1; }
 
-Plan make_plan(uint64_t rows, uint32_t cols, int es, bool aligned) {
+Plan make_plan(uint64_t rows, uint32_t cols, int es, bool aligned, int sm = sm_count()) {
   Plan p;
-  const uint64_t sms = static_cast<uint64_t>(sm_count());
+  const uint64_t sms = static_cast<uint64_t>(sm);
   const uint64_t row_bytes = static_cast<uint64_t>(cols) * es;
   if (aligned && cols <= 16384) {
     // 8 values per thread in groups of 8 to 32 threads, then 16, then (rows of more than 8192 columns) 32
@@ -683,6 +683,12 @@ uint64_t layernorm_backward_workspace(uint64_t rows, uint32_t cols, int elem_byt
   const Plan a = make_plan(rows, cols, elem_bytes, false), b = make_plan(rows, cols, elem_bytes, true);
   const uint64_t na = a.row_sums_bytes + a.partial_bytes, nb = b.row_sums_bytes + b.partial_bytes;
   return na > nb ? na : nb;
+}
+
+void layernorm_backward_plan(uint64_t rows, uint32_t cols, int elem_bytes, int aligned, int sms, uint32_t* out) {
+  const Plan p = make_plan(rows, cols, elem_bytes, aligned != 0, sms);
+  const uint32_t v[8] = {static_cast<uint32_t>(p.kind), static_cast<uint32_t>(p.values), p.tpr, p.groups, p.per_group, p.stages, p.plane, p.parts};
+  for (int i = 0; i < 8; ++i) out[i] = v[i];
 }
 
 int layernorm_backward_status(int* out) {

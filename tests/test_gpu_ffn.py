@@ -198,6 +198,58 @@ def test_gradients_against_differences(tcab_lib, cuda):
     differences(plain, [at[0], at[1], at[3]], [got["da"], got["db"], got["dbias"]], 4)
 
 
+def test_activation_values_and_slopes(tile, cuda):
+    """Over the whole range of arguments: an empty contraction stores act(bias), one row's dbias is the slope in fp32."""
+    import tcacomp_b200 as T
+    grid = torch.cat([torch.linspace(-40, 40, 3997, device="cuda"), torch.logspace(-30, 38, 200, device="cuda"),
+                      -torch.logspace(-30, 38, 200, device="cuda"), torch.tensor([0.0, -0.0, float("nan")], device="cuda")])
+    n = grid.numel()
+    assert n % 8 == 0
+    none = torch.empty((1, 0), device="cuda", dtype=BF)
+    for act in ("relu", "silu", "gelu", "gelu_tanh"):
+        want = R.act(grid.double(), act)
+        got = T.gemm_bias_act_residual(none, torch.empty((0, n), device="cuda", dtype=BF), grid, act=act)[0]
+        bound = R.ACT_ERR * (1 + want.abs())
+        # values below fp32's smallest normal number may be flushed to zero
+        R.check(got, want, bound + R.H16 * (want.abs() + bound) + 2.0 ** -126, f"{act}")
+        z = grid.to(BF)
+        wslope = R.slope(z.double(), act)
+        if act == "relu":
+            wslope[torch.isnan(z)] = 0  # a comparison with NaN is false
+        a, b = torch.zeros((1, 8), device="cuda", dtype=BF), torch.zeros((8, n), device="cuda", dtype=BF)
+        got = T.gemm_bias_act_backward(torch.ones((1, n), device="cuda", dtype=BF), a, b, z.view(1, n), act, want=("dbias",))["dbias"]
+        # beyond 1e3 every slope here is 0 or 1 to the last bit (the reference's own formula overflows there)
+        far = z.double().abs() > 1e3
+        wslope = torch.where(far, (z > 0).double(), wslope)
+        R.check(got, wslope, R.ACT_ERR * (1 + z.double().abs().clamp(max=40)), f"slope of {act}")
+
+
+def test_two_threads_on_their_own_streams(tcab_lib, cuda):
+    """Host threads that call at the same time, each on a stream of its own: the results are those of calls alone."""
+    import threading
+
+    import tcacomp_b200 as T
+    sets = [(rnd(200, 256, seed=40 + i), rnd(256, 520, seed=50 + i), rnd(200, 520, seed=60 + i)) for i in range(2)]
+    want = [(T.gemm_bias_act_residual(a, b, None, dc, "silu"), T.gemm_bias_act_backward(dc, a, b, dc, "silu")) for a, b, dc in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        a, b, dc = sets[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                c = T.gemm_bias_act_residual(a, b, None, dc, "silu")
+                g = T.gemm_bias_act_backward(dc, a, b, dc, "silu")
+            torch.cuda.current_stream().synchronize()
+        if not torch.equal(c, want[i][0]) or any(not torch.equal(g[k], want[i][1][k]) for k in g):
+            bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad and T.device_status() == 0
+
+
 def test_empty_extents(tcab_lib, cuda):
     import tcacomp_b200 as T
     bias = torch.linspace(-1, 1, 16, device="cuda")
