@@ -283,7 +283,9 @@ TCAB_API int tcab_gemm_bias_act(const tcab_tensor* a, const tcab_tensor* b, cons
  * A feed-forward sublayer and its training step. The reference has no backward passes and no such layer; these stand
  * beside tcab_layernorm_rows and tcab_gemm_bias_act and follow their rules. None of them allocates: a backward pass takes
  * a workspace of at least the bytes its _workspace function gives (16-byte aligned device memory on the current device,
- * free to be reused once the call's work on the stream is done; two calls that may overlap on the GPU need one each).
+ * free to be reused once the call's work on the stream is done; two calls that may overlap on the GPU need one each; it
+ * must not overlap a tensor of the call). The innermost extent of a row form and every extent of a contraction is below
+ * 2^31.
  * An output must not overlap another output or an input; where a comment names an input that an output may be, the two
  * must start at the same address. Every sum is fp32 and taken in a fixed order: the same call gives the same bits.
  * --------------------------------------------------------------------------------------------------- */

@@ -272,6 +272,25 @@ int need_disjoint(const char* op, const Named* outs, int n_outs, const Named* in
   return TCAB_OK;
 }
 
+// A workspace against the tensors of its call.
+int need_apart(const char* op, const void* ws, uint64_t bytes, const Named* ts, int n) {
+  const uintptr_t w = reinterpret_cast<uintptr_t>(ws);
+  for (int i = 0; i < n && ws != nullptr && bytes > 0; ++i) {
+    if (ts[i].t == nullptr) continue;
+    const uintptr_t p = reinterpret_cast<uintptr_t>(ts[i].t->data);
+    const uint64_t size = tensor_bytes(ts[i].t);
+    if (size > 0 && (p >= w ? p - w < bytes : w - p < size))
+      return fail(TCAB_ERR_INVALID_ARG, "%s: the workspace overlaps %s", op, ts[i].name);
+  }
+  return TCAB_OK;
+}
+
+// Extents are walked in 32 bits, a stride past the end included, and are coordinates of tensor maps.
+int need_extent(const char* op, const char* name, uint32_t extent) {
+  if (extent > 0x7fffffffu) return fail(TCAB_ERR_TOO_LARGE, "%s: an extent of %s is 2^31 or more", op, name);
+  return TCAB_OK;
+}
+
 // mean / rstd of x's rows: f32, the extents of x without the innermost one (rank-1 x: extent 1).
 int check_row_stats(const char* op, const char* name, const tcab_tensor* t, const tcab_tensor* x) {
   TCAB_TRY(check_tensor(op, name, t));
@@ -295,6 +314,7 @@ int check_norm_rows(const char* op, const tcab_tensor* x) {
   TCAB_TRY(check_tensor(op, "x", x));
   if (x->dtype != TCAB_F32 && x->dtype != TCAB_BF16) return fail(TCAB_ERR_DTYPE, "%s: x must be f32 or bf16", op);
   if (x->dims[x->rank - 1] == 0) return fail(TCAB_ERR_SHAPE, "%s: the innermost extent of x must be positive", op);
+  TCAB_TRY(need_extent(op, "x", x->dims[x->rank - 1]));
   return need_elem_align(op, "x", x, x->dtype == TCAB_F32 ? 4 : 2);
 }
 
@@ -335,6 +355,10 @@ int check_contraction(const char* op, const char* an, const tcab_tensor* a, cons
   *m = a->dims[0];
   *k = a->dims[1];
   *n = b->dims[1];
+  for (int i = 0; i < 2; ++i) {
+    TCAB_TRY(need_extent(op, an, a->dims[i]));
+    TCAB_TRY(need_extent(op, bn, b->dims[i]));
+  }
   if (*k % 8 != 0 || *n % 8 != 0)
     return fail(TCAB_ERR_ALIGNMENT, "%s: K and N must be multiples of 8 (16-byte rows for the tensor maps)", op);
   TCAB_TRY(need_elem_align(op, an, a, 16));
@@ -891,6 +915,8 @@ int tcab_layernorm_rows_backward(const tcab_tensor* dy, const tcab_tensor* x, co
   const Named ins[] = {{"dy", dy}, {"x", x}, {"gamma", gamma}, {"mean", mean}, {"rstd", rstd}};
   const tcab_tensor* may_be[] = {dy, x};
   TCAB_TRY(need_disjoint(op, outs, 3, ins, 5, may_be, 2));
+  TCAB_TRY(need_apart(op, workspace, workspace_bytes, outs, 3));
+  TCAB_TRY(need_apart(op, workspace, workspace_bytes, ins, 5));
   TCAB_TRY(have_device(op));
   TCAB_TRY(check_workspace(op, workspace, workspace_bytes, tcab_layernorm_rows_backward_workspace(x)));
   const uint64_t rows = count(x, 0, x->rank - 1);
@@ -951,6 +977,8 @@ int tcab_gemm_bias_act_backward(const tcab_tensor* dc, const tcab_tensor* a, con
   TCAB_TRY(check_bias_opt(op, "dbias", dbias, n));
   const Named outs[] = {{"da", da}, {"db", db}, {"dbias", dbias}}, ins[] = {{"dc", dc}, {"a", a}, {"b", b}, {"preact", preact}};
   TCAB_TRY(need_disjoint(op, outs, 3, ins, 4));
+  TCAB_TRY(need_apart(op, workspace, workspace_bytes, outs, 3));
+  TCAB_TRY(need_apart(op, workspace, workspace_bytes, ins, 4));
   TCAB_TRY(have_device(op));
   TCAB_TRY(check_workspace(op, workspace, workspace_bytes, tcab_gemm_bias_act_backward_workspace(m, n, act, dbias != nullptr)));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1049,6 +1077,8 @@ int tcab_gated_gemm_backward(const tcab_tensor* dh, const tcab_tensor* x, const 
   const Named outs[] = {{"dx", dx}, {"dw_gate", dw_gate}, {"dw_up", dw_up}, {"dbias_gate", dbias_gate}, {"dbias_up", dbias_up}};
   const Named ins[] = {{"dh", dh}, {"x", x}, {"w_gate", w_gate}, {"w_up", w_up}, {"gate", gate}, {"up", up}};
   TCAB_TRY(need_disjoint(op, outs, 5, ins, 6));
+  TCAB_TRY(need_apart(op, workspace, workspace_bytes, outs, 5));
+  TCAB_TRY(need_apart(op, workspace, workspace_bytes, ins, 6));
   TCAB_TRY(have_device(op));
   TCAB_TRY(check_workspace(op, workspace, workspace_bytes, tcab_gated_gemm_backward_workspace(m, n, dbias_gate != nullptr)));
   if (dx == nullptr && dw_gate == nullptr && dbias_gate == nullptr) return TCAB_OK;

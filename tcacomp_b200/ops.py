@@ -489,6 +489,8 @@ class _At:
 
 
 def _at(dev: int, stream: Optional[torch.cuda.Stream]):
+    if stream is not None and stream.device_index != dev:
+        raise ValueError(f"the stream is on cuda:{stream.device_index} but the first operand is on cuda:{dev}")
     if stream is None and dev == torch._C._cuda_getDevice():
         return _ALREADY_CURRENT
     return _At(dev, stream)

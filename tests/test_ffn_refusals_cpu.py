@@ -172,3 +172,45 @@ def test_without_a_device_and_python_arguments(tcab_lib):
     S = Space()
     assert call(tcab_lib, "tcab_gated_gemm", [S(5, 64), S(64, 40), S(64, 40), None, None, 2, None, None, S(5, 40), None]) == _lib.ERR_CUDA
     assert call(tcab_lib, "tcab_gemm_bias_act_residual", [S(5, 64), S(64, 40), None, None, 0, None, S(5, 40), None]) == _lib.ERR_CUDA
+
+
+def test_workspace_apart_from_the_tensors(tcab_lib):
+    """A workspace that begins or ends inside a tensor of the call is refused; one that only touches it gets further."""
+    from tcacomp_b200 import _lib
+    L, S = tcab_lib, Space()
+    dc, a, b, z, da, db = S(5, 40), S(5, 64), S(64, 40), S(5, 40), S(5, 64), S(64, 40)
+    x, g, mean, rstd, dx = S(4, 64), S(64), S(4, dtype=0), S(4, dtype=0), S(4, 64)
+    dg, dbt = S(64, dtype=0), S(64, dtype=0)
+    h, gate, up, w1, w2, dw1, dw2 = S(5, 40), S(5, 40), S(5, 40), S(64, 40), S(64, 40), S(64, 40), S(64, 40)
+
+    def gemm(ws, n):
+        return call(L, "tcab_gemm_bias_act_backward", [dc, a, b, z, 3, da, db, None, ws, n, None])
+
+    def norm(ws, n):
+        return call(L, "tcab_layernorm_rows_backward", [dx, x, g, mean, rstd, dx, dg, dbt, ws, n, None])
+
+    def gated(ws, n):
+        return call(L, "tcab_gated_gemm_backward", [h, a, w1, w2, gate, up, 2, da, dw1, dw2, None, None, ws, n, None])
+
+    for fn, tensors in ((gemm, {"dc": dc, "a": a, "preact": z, "db": db}), (norm, {"x": x, "rstd": rstd, "dgamma": dg}),
+                        (gated, {"dh": h, "up": up, "w_up": w2, "dx": da, "dw_up": dw2})):
+        for name, t in tensors.items():
+            size = 4 * t.dims[0] if t.rank == 1 else 2 * t.dims[0] * t.dims[1]
+            for ws in (t.data, t.data - 4080, t.data + size - 16):
+                assert fn(ws, 4096) == _lib.ERR_INVALID_ARG and f"workspace overlaps {name}" in message(L), (name, ws - t.data)
+            for ws in (t.data - 4096, t.data + size):
+                fn(ws, 16)
+                assert "workspace overlaps" not in message(L)
+
+
+def test_extents_of_31_bits(tcab_lib):
+    """With an empty contraction an extent may pass 31 bits without a tensor passing 2^32 elements."""
+    from tcacomp_b200 import _lib
+    L = tcab_lib
+    far = 1 << 40
+    n = (1 << 31) + 8
+    a, b, c = T_((1, 0), 1, 0), T_((0, n), 1, 0), T_((1, n), 1, far)
+    assert call(L, "tcab_gemm_bias_act_residual", [a, b, None, None, 0, None, c, None]) == _lib.ERR_TOO_LARGE and "2^31" in message(L)
+    assert call(L, "tcab_gated_gemm", [a, b, b, None, None, 2, None, None, c, None]) == _lib.ERR_TOO_LARGE
+    x, y, g, st = T_((1, n), 1, far), T_((1, n), 1, 2 * far), T_((n,), 1, 3 * far), T_((1,), 0, 4 * far)
+    assert call(L, "tcab_layernorm_rows_stats", [x, g, T_((n,), 1, 5 * far), 1e-5, y, st, T_((1,), 0, 6 * far), None]) == _lib.ERR_TOO_LARGE

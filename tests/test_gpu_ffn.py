@@ -403,3 +403,64 @@ def test_a_training_step_captured_and_replayed(tcab_lib, cuda):
         assert torch.equal(out, o) and all(torch.equal(grads[name], g[name]) for name in g)
     assert torch.equal(out, want[1][0]) and torch.equal(eager["db"], want[2][1]["dw_down"])
     assert T.device_status() == 0
+
+
+def test_a_captured_fork_and_join(tcab_lib, cuda):
+    """A capture whose calls wait for events of another stream: both branches of a sublayer and what joins them."""
+    import tcacomp_b200 as T
+    p = block_params(256, 520)
+    x, y = rnd(130, 256, seed=50), rnd(130, 256, seed=51)
+    want = T.gemm_bias_act_residual(block_forward(T, p, x)[0], p["w_gate"], None, block_forward(T, p, y)[1][3], "none")
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            gate = block_forward(T, p, y)[1][3]
+        out = block_forward(T, p, x)[0]
+        main.wait_stream(side)
+        got = T.gemm_bias_act_residual(out, p["w_gate"], None, gate, "none")
+    for _ in range(5):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_offsets_past_32_bits(tcab_lib, cuda):
+    """Tensors of 4.29e9 elements, 8.6 GB each: the last row, some in the middle, the last columns."""
+    import tcacomp_b200 as T
+    m, k, n = 65528, 16, 65536
+    a, b, bias = rnd(m, k, seed=1), rnd(k, n, seed=2), torch.randn(n, device="cuda")
+    c, z = torch.empty(m, n, device="cuda", dtype=BF), torch.empty(m, n, device="cuda", dtype=BF)
+    T.gemm_bias_act_residual(a, b, bias, None, "silu", out=c, preact=z)
+    rows = [0, 1, 16384, 32767, 32768, 49999, m - 2, m - 1]
+    want, e = R.project(a[rows], b, bias)
+    R.check(z[rows], want, e + R.H16 * (want.abs() + e), "preact")
+    want = R.act(want, "silu")
+    bound = R.SLOPE * e + R.ACT_ERR * (1 + want.abs())
+    R.check(c[rows], want, bound + R.H16 * (want.abs() + bound), "c")
+    # dz = z silu'(z), with z in dc's place too: rounded once, then contracted over the 65536 columns
+    got = T.gemm_bias_act_backward(z, a, b, z, "silu", want=("da",))["da"]
+    zr = z[rows].double()
+    dz = zr * R.slope(zr, "silu")
+    e_dz = zr.abs() * R.ACT_ERR * (1 + R.act(zr, "silu").abs()) + R.H32 * dz.abs()
+    e_dz = e_dz + R.H16 * (dz.abs() + e_dz)
+    want, size = dz @ b.double().t(), (dz.abs() + e_dz) @ b.double().abs().t()
+    bound = e_dz @ b.double().abs().t() + (n + 2) * 2.0 ** -23 * size
+    R.check(got[rows], want, bound + R.H16 * (want.abs() + bound), "da")
+    del c, z
+    torch.cuda.empty_cache()
+
+
+def test_a_stream_of_another_device(tcab_lib, cuda):
+    import types
+
+    import tcacomp_b200 as T
+    other = types.SimpleNamespace(device_index=1, cuda_stream=0)
+    a = rnd(8, 16, seed=1)
+    for call in (lambda: T.gemm_bias_act_residual(a, rnd(16, 8, seed=2), act="none", stream=other),
+                 lambda: T.gated_gemm(a, rnd(16, 8, seed=2), rnd(16, 8, seed=3), stream=other),
+                 lambda: T.layernorm_rows_stats(a, a[0], a[1], stream=other)):
+        with pytest.raises(ValueError, match="stream is on cuda:1"):
+            call()

@@ -170,3 +170,26 @@ def test_captured_and_replayed_beside_another_stream(tcab_lib, cuda):
     torch.cuda.synchronize()
     for got, w in zip(outs + [eager], want):
         assert all(torch.equal(p, q) for p, q in zip(got, w))
+
+
+@pytest.mark.parametrize("rows,cols", [(1048568, 4096), (65528, 65536)])
+def test_offsets_past_32_bits(tcab_lib, cuda, rows, cols):
+    """Tensors of 4.29e9 elements: rows at both ends and in the middle, dx written over dy."""
+    import tcacomp_b200 as T
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    x = torch.randn(rows, cols, device="cuda", generator=g, dtype=BF)
+    gamma = torch.randn(cols, device="cuda", generator=g, dtype=BF)
+    dy, mean, rstd = T.layernorm_rows_stats(x, gamma, gamma, 1e-5)
+    pick = [0, 1, rows // 4, rows // 2 - 1, rows // 2, rows - 2, rows - 1]
+    wy, wm, wr, ey, em, er = R.layernorm(x[pick], gamma, gamma, 1e-5)
+    few = dy[pick].clone()
+    R.check(few, wy, ey + R.H16 * (wy.abs() + ey), "y")
+    R.check(mean[pick], wm, em + R.H32 * wm.abs(), "mean")
+    R.check(rstd[pick], wr, er, "rstd")
+    dx, dgamma, dbeta = T.layernorm_rows_backward(dy, x, gamma, mean, rstd, dx=dy)
+    wx, _, _, ex, _, _ = R.layernorm_grads(few, x[pick], gamma, mean[pick], rstd[pick])
+    R.check(dx[pick], wx, ex + R.H16 * (wx.abs() + ex), "dx")
+    assert torch.isfinite(dgamma).all() and torch.isfinite(dbeta).all()
+    del x, dx, dy
+    torch.cuda.empty_cache()
