@@ -985,12 +985,15 @@ int tcab_gemm_bias_act_backward(const tcab_tensor* dc, const tcab_tensor* a, con
   const __nv_bfloat16* dz = bf16_of(dc);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const bool contract = da != nullptr || db != nullptr;
+  bool beside = false;  // the last launch of this call so far, if there is one, does not write dz
   if (act != TCAB_ACT_NONE && (contract || dbias != nullptr)) {
     __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(ws);
     TCAB_TRY(launch_act_backward(op, act, dz, bf16_of(preact), contract ? to : nullptr, f32_of(dbias), m, n, ws + round256(2ull * m * n), s));
     dz = to;
+    beside = dbias != nullptr && n > 0 && act_backward_finishes(m, n, 0);
   } else if (dbias != nullptr) {
     TCAB_TRY(launch_act_backward(op, TCAB_ACT_NONE, dz, nullptr, nullptr, f32_of(dbias), m, n, ws, s));
+    beside = n > 0;
   }
   if (da != nullptr) {
     FfnProblem p;
@@ -1000,7 +1003,9 @@ int tcab_gemm_bias_act_backward(const tcab_tensor* dc, const tcab_tensor* a, con
     p.M = m;
     p.N = k;
     p.K = n;
+    p.beside = beside;
     TCAB_TRY(launch_ffn_gemm(op, kFfnDx, p, s));
+    beside = beside || (m > 0 && k > 0);
   }
   if (db != nullptr) {
     FfnProblem p;
@@ -1010,6 +1015,7 @@ int tcab_gemm_bias_act_backward(const tcab_tensor* dc, const tcab_tensor* a, con
     p.M = k;
     p.N = n;
     p.K = m;
+    p.beside = beside;
     TCAB_TRY(launch_ffn_gemm(op, kFfnDw, p, s));
   }
   return TCAB_OK;
@@ -1089,6 +1095,7 @@ int tcab_gated_gemm_backward(const tcab_tensor* dh, const tcab_tensor* x, const 
   __nv_bfloat16* dup = reinterpret_cast<__nv_bfloat16*>(ws + plane);
   TCAB_TRY(launch_gated_backward(op, act, bf16_of(dh), bf16_of(gate), bf16_of(up), dgate, dup, f32_of(dbias_gate), f32_of(dbias_up),
                                  m, n, ws + 2 * plane, s));
+  bool beside = dbias_gate != nullptr && n > 0;  // the last launch of this call so far, if there is one, writes neither
   if (dx != nullptr) {
     FfnProblem p;
     p.a[0] = dgate;
@@ -1099,7 +1106,9 @@ int tcab_gated_gemm_backward(const tcab_tensor* dh, const tcab_tensor* x, const 
     p.M = m;
     p.N = k;
     p.K = n;
+    p.beside = beside;
     TCAB_TRY(launch_ffn_gemm(op, kFfnDx, p, s));
+    beside = beside || (m > 0 && k > 0);
   }
   if (dw_gate != nullptr) {
     FfnProblem p;
@@ -1111,6 +1120,7 @@ int tcab_gated_gemm_backward(const tcab_tensor* dh, const tcab_tensor* x, const 
     p.M = k;
     p.N = n;
     p.K = m;
+    p.beside = beside;
     TCAB_TRY(launch_ffn_gemm(op, kFfnDw, p, s));
   }
   return TCAB_OK;

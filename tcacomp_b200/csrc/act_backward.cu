@@ -167,7 +167,7 @@ int launch(const char* op, const __nv_bfloat16* in0, const __nv_bfloat16* in1, c
   const uint32_t parts = row_parts(rows, cols);
   const dim3 grid((cols + kStripCols - 1) / kStripCols, parts);
   float* sum = static_cast<float*>(ws);
-  const bool direct = sums && !GATED && parts == 1;  // one partial row: it is the result
+  const bool direct = sums && !act_backward_finishes(rows, cols, GATED);  // one partial row: it is the result
   if (direct) sum = dbias0;
   if (sums) launch_pdl(act_backward_kernel<ACT, GATED, true>, grid, dim3(256), 0, s, in0, in1, in2, out0, out1, sum, rows, cols);
   else launch_pdl(act_backward_kernel<ACT, GATED, false>, grid, dim3(256), 0, s, in0, in1, in2, out0, out1, static_cast<float*>(nullptr), rows, cols);
@@ -182,6 +182,8 @@ int launch(const char* op, const __nv_bfloat16* in0, const __nv_bfloat16* in1, c
 }
 
 }  // namespace
+
+bool act_backward_finishes(uint32_t rows, uint32_t cols, int gated) { return gated || row_parts(rows, cols) > 1; }
 
 uint64_t act_backward_workspace(uint32_t rows, uint32_t cols, int gated) {
   return static_cast<uint64_t>(row_parts(rows, cols)) * (gated ? 2 : 1) * cols * sizeof(float);

@@ -127,6 +127,7 @@ int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t 
   args.bias[1] = p.bias[1];
   args.residual = p.residual;
   args.save = p.z[0] != nullptr ? 1 : 0;
+  args.beside = p.beside ? 1 : 0;
   const int nb = p.b[1] != nullptr ? 2 : 1;
   if (p.K > 0) {
     if (form == kFfnDw) {

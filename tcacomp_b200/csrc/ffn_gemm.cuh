@@ -41,6 +41,7 @@ struct FfnArgs {
   uint32_t M, N, K;
   uint32_t pairs;  // Dx: contracted pairs (1, 2); Dw: outputs (1, 2)
   int save;        // Fwd, Gated: also store the projections
+  int beside;      // FfnProblem::beside
 };
 
 // What a translation unit of this kernel family gives: an instance, its dynamic shared memory and its status word
@@ -139,7 +140,7 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
   if (PAIR) ptx::cluster_wait();  // the peer's barriers must be initialised before anything of this CTA can signal them
   ptx::tc_fence_after();
   const uint32_t tmem_base = tmem_base_slot;
-  ptx::pdl_wait();
+  if (!args.beside) ptx::pdl_wait();
   ptx::pdl_launch();
 
   // Register split: 384 threads x 168 at launch = 64,512; 128 x 40 + 256 x 224 = 62,464 afterwards.
@@ -511,6 +512,7 @@ ffn_gemm_kernel(const __grid_constant__ FfnArgs args) {
     else ptx::tmem_dealloc(tmem_base, 512);
   }
   if (threadIdx.x == 0 && abort_flag != 0) g_ffn_status = 1;
+  if (args.beside) ptx::pdl_wait();
 }
 
 // The kernel of a form, an activation and a tile shape.

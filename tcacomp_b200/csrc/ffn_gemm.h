@@ -25,6 +25,11 @@ struct FfnProblem {
   const __nv_bfloat16* residual = nullptr;
   uint32_t M = 0, N = 0, K = 0;
   int act = TCAB_ACT_NONE;
+  // The launch before this one on the stream belongs to the same call and writes none of the operands. The kernel then runs
+  // beside it (515 x 1032 x 2056 backward: the second product on the SMs that the first leaves) and waits for it at its own
+  // end, so that whoever waits for this kernel has waited for both. What the operands need was complete before: a kernel
+  // lets its successor start only when it runs itself, and the first of a call runs on only after everything before it.
+  bool beside = false;
 };
 
 int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t s);
@@ -46,6 +51,8 @@ void ffn_plan(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int 
 
 // dz = dc * act'(z) (gated: dgate = dh * up * act'(gate), dup = dh * act(gate)), with the column sums of each where
 // wanted (act_backward.cu). dz may be null (column sums alone; act none). Partials of the sums go to `ws`.
+// Whether column sums take a second launch, behind the one that writes dz.
+bool act_backward_finishes(uint32_t rows, uint32_t cols, int gated);
 uint64_t act_backward_workspace(uint32_t rows, uint32_t cols, int gated);
 int launch_act_backward(const char* op, int act, const __nv_bfloat16* dc, const __nv_bfloat16* z, __nv_bfloat16* dz,
                         float* dbias, uint32_t rows, uint32_t cols, void* ws, cudaStream_t s);

@@ -78,6 +78,7 @@ int launch_ffn_small(const char* op, int form, const FfnProblem& p, cudaStream_t
   args.blocks_per_range = plan.blocks_per_range;
   args.stages = stages;
   args.act = p.act;
+  args.beside = p.beside ? 1 : 0;
   args.residual = p.residual;
   for (int i = 0; i < 2; ++i) {
     args.c[i] = p.c[i];

@@ -40,6 +40,7 @@ struct FfnSmallArgs {
   uint32_t ks, blocks_per_range;  // CTAs per tile (1, 2, 4, 8), K blocks of each
   uint32_t stages;
   int act;
+  int beside;  // FfnProblem::beside
 };
 
 struct FfnSmallKernel {
@@ -141,7 +142,7 @@ ffn_small_kernel(const __grid_constant__ FfnSmallArgs args) {
     ptx::mbar_init(ptx::smem_u32(&bar_received), ks);
     ptx::fence_barrier_init();
     ptx::fence_proxy_async();
-    ptx::pdl_wait();
+    if (!args.beside) ptx::pdl_wait();
     // the first blocks are under way before the TMEM allocation and the barrier below; the others follow it: a full ring
     // of copies from one thread takes 1,500 cycles
     for (uint32_t i = 0; i < num_kb && i < first_blocks; ++i) issue(i, i);
@@ -190,7 +191,7 @@ ffn_small_kernel(const __grid_constant__ FfnSmallArgs args) {
     }
   }
   __syncwarp();
-  ptx::pdl_wait();  // every thread: what follows reads and writes global memory
+  if (!args.beside) ptx::pdl_wait();  // every thread: what follows reads and writes global memory
   const uint32_t live_rows = min(static_cast<uint32_t>(TM), M - m0);
   // A lane of TMEM is a column of the tile. Its owner is the CTA that stores it; there it is column `mine` of the range.
   const uint32_t col = (static_cast<uint32_t>(warp) & 3u) * 32 + lane, per = TN / ks;  // columns per owner (of each projection)
@@ -278,6 +279,7 @@ ffn_small_kernel(const __grid_constant__ FfnSmallArgs args) {
     *reinterpret_cast<uint4*>(args.c[which] + at) = pack8(v[0]);
   }
   if (threadIdx.x == 0 && abort_flag != 0) g_small_status = 1;
+  if (args.beside) ptx::pdl_wait();
   if (ks > 1) {
     __syncwarp();
     ptx::cluster_wait();  // no CTA leaves while a peer may still signal it
