@@ -20,7 +20,7 @@
 // Everything works on eight values at a time, step by step over all eight, multiply-adds two at a time (FFMA2): an
 // epilogue has two warps per scheduler, so one value's chain of a reciprocal, an exp2 and a dozen multiply-adds has to
 // overlap with its neighbours'. An 8192^3 product with gelu (TFLOP/s): one value after the other with erff 1,090, with
-// the tail form 1,250, eight at a time 1,3xx; without an activation 1,400.
+// the tail form 1,250, eight at a time 1,360; without an activation 1,400-1,435.
 #pragma once
 
 #include "f32x2.cuh"

@@ -47,11 +47,13 @@ constexpr int kShapes = 3, kCtas[kShapes] = {2, 2, 1}, kRows[kShapes] = {512, 25
 // The kernel: a tile shape of the persistent one, or kShapes for ffn_small.cuh. An estimate in microseconds per shape --
 // what a launch costs before its first and behind its last block, rounds over the SMs (pairs of SMs), blocks of 64 per
 // round -- fitted to outputs of 1003 x 2728, 1024 x 2816 and 512 x 4096 over 64 ... 2048 (graphs of launches):
-//   512 x 256 on pairs 8.3 + 0.49 per block, 256 x 256 on pairs 5.8 + 0.30, 128 x 128 3.6 + 0.30 (its two operand tiles per
-//   128 x 128 products are at the shared-memory limit), against 3.1-3.7 for a library product's launch.
+//   512 x 256 on pairs 8.3 + 0.49 per block, 256 x 256 on pairs 5.8 + 0.30, 128 x 128 3.6 + 0.25.
+// Both sides of it, us for 512 x 256, 256 x 256, 128 x 128, the small kernel (the choice first): 512 x 4096 x 4096 20.1 for
+// 128 x 128, against 42.5, 22.5, 26.5; 1003 x 1000 x 2728 11.2 for 256 x 256, against 17.3, 16.7, 24.9; 2048 x 4096 x 4096
+// 46.5 for 512 x 256, against 47.8, 77.4, 103; 256 x 4096 x 4096 16.1 for the small one, against 41.8, 22.3, 19.0.
 // Over many rounds the 512 x 256 tile wins (8192^3: 1,395 TFLOP/s against 1,305 for 256 x 256): it moves the fewest bytes.
 int choose(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sm) {
-  static const double kFixed[kShapes] = {8.3, 5.8, 3.6}, kBlock[kShapes] = {0.49, 0.30, 0.30}, kEpilogue[kShapes] = {4.0, 2.2, 1.0};
+  static const double kFixed[kShapes] = {8.3, 5.8, 3.6}, kBlock[kShapes] = {0.49, 0.30, 0.25}, kEpilogue[kShapes] = {4.0, 2.2, 1.0};
   const uint64_t sms = static_cast<uint64_t>(sm);
   const uint64_t outs = form == kFfnDw ? pairs : 1, blocks = (static_cast<uint64_t>(k) + 63) / 64 * (form == kFfnDx ? pairs : 1);
   int best = kShapes;

@@ -9,17 +9,26 @@
 //   Dx      [M, K] (twice)         [N, K] (twice), K-major                 BN rows; the K loop runs over both pairs
 //   Dw      [K, M], M-major        [K, N] (twice), N-major                 BN columns; tiles of the second output follow
 //
-// A tile is 256 x 256 on a pair of CTAs (cta_group::2: each loads its 128 rows of a and half of b's columns, the
-// leader issues the MMAs), or 128 x 256 or 128 x 128 on one CTA. Roles: warp 0 (one lane) is the TMA producer, warp 1
-// (one lane) issues the MMAs, warps 4-11 are the epilogue (and take most of the registers). A K block is 64 wide; a CTA's accumulator is 128 x BN, and TMEM
-// holds 512 / BN of them in a ring, so that the epilogue of a tile -- activations, products, residuals, up to three stored
-// matrices -- runs under the K loop of the next. It takes 32 columns at a time, with the next 32 under way from TMEM.
+// A tile is 512 x 256 or 256 x 256 on a pair of CTAs (cta_group::2: each loads its rows of a and half of b's columns, the
+// leader issues the MMAs), or 128 x 128 on one CTA. Roles: warp 0 (one lane) is the TMA producer, warp 1 (one lane) issues
+// the MMAs, warps 4-11 are the epilogue and take most of the registers. A K block is 64 wide; an accumulator is 128 rows x
+// BN columns per CTA, and TMEM holds 512 / BN of them. With 256 x 256 and 128 x 128 they form a ring, so that the epilogue
+// of a tile -- activations, products, residuals, up to three stored matrices -- runs under the K loop of the next. With
+// 512 x 256 a tile takes both accumulators: the first is read into registers and handed back before anything is computed,
+// the second follows block by block.
+//
+// Bound: the tensor pipe up to where the power limit lowers the clock; from some thousand rows on, energy per product.
+// 8192^3 without an activation: 512 x 256 1,395 TFLOP/s (tensor pipe 85 % busy at 1,342 MHz), 256 x 256 1,305 (92 % at
+// 1,170: it moves half as many bytes again). Two K blocks share a ring stage where there is room: a stage's wait, signal
+// and commit cost 15 % of the K loop with one block each (256 x 256 .80 -> .91 busy; 128 x 128 tiles, 512 x 4096 x 4096:
+// 25.7 -> 20.1 us, from there on L2: 16 TB/s of operand tiles). 256 x 128 tiles on pairs were no faster than 128 x 128
+// (20.2 us there, 14.2 against 11.1 for 256 x 256 at 1003 x 1000 x 2728) and are not built.
 //
 // Results leave as 32 x 32 boxes: a lane holds a row of 32 columns, the box turns in a 2 KB buffer of the warp, and four
 // 16-byte stores per lane write 64-byte row segments. (TMA stores from two such buffers were measured first: about 1,000
 // cycles per box, most of them waiting for a buffer to be read, against 250; where a CTA has one tile, nothing hides
-// that.) A residual takes the same way in. Loads past an edge read zeros. Every wait is bounded (sm100_ptx.cuh); a wait that gives up ends the kernel
-// with a status word.
+// that.) A residual takes the same way in. Loads past an edge read zeros. Every wait is bounded (sm100_ptx.cuh); a wait
+// that gives up ends the kernel with a status word.
 #pragma once
 
 #include "activation.cuh"
@@ -525,7 +534,7 @@ FfnKernel ffn_kernel_of(int shape) {
   switch (shape) {
     case 0: return ffn_kernel_shape<FORM, ACT, 2, 2, 256, 1>();
     case 1: return ffn_kernel_shape<FORM, ACT, 2, 1, 256, 2>();
-    default: return ffn_kernel_shape<FORM, ACT, 1, 1, 128, 1>();
+    default: return ffn_kernel_shape<FORM, ACT, 1, 1, 128, 2>();
   }
 }
 

@@ -19,6 +19,13 @@
 // and arrives on their barriers, and an owner adds what it received in ascending order of the ranges, then bias,
 // activation, product, residual. The sums have a fixed order; nothing is atomic. Cluster barriers remain only for
 // lifetimes, arrived at early and waited for late.
+//
+// Measured in graphs of launches: one token 4096 x 4096 7.7-9.8 us (8 ranges), 16 tokens through two weights of 4096 x 11008
+// 33.4 us (5.4 TB/s of weights, 82 % of the copy rate), 64 rows 9.2, 128 rows 11.0 us.
+//
+// The CTAs of a cluster wait for one another while each holds TMEM, so an SM's 512 columns must suffice for all CTAs that
+// fit on it: at most 1.3 columns per KB of shared memory of any kernel here beside this one (128 of 97 KB, 256 of 193 KB
+// in gemm_bias_act.cu), 300 in all; kernels that take all 512 columns leave no room for a second CTA.
 #pragma once
 
 #include "activation.cuh"
