@@ -149,20 +149,20 @@ def load() -> C.CDLL:
     return lib
 
 
-_PACKED: dict = {}
-
-
-def packed(name: str):
-    """The function `name` taking its tensors as bytes objects that hold a tcab_tensor (or None), for operators of many
-    tensors: a prototype of its own beside the one load() binds."""
-    fn = _PACKED.get(name)
-    if fn is None:
-        restype, argtypes = next((r, a) for n, r, a in SYMBOLS if n == name)
-        fn = load()[name]  # a new function object: load()'s keeps its own argument types
-        fn.restype = restype
-        fn.argtypes = [C.c_char_p if a is C.POINTER(Tensor) else a for a in argtypes]
-        _PACKED[name] = fn
-    return fn
+def load_calls(view):
+    """The extension module _calls (csrc/torch/calls.cpp) bound to the loaded library; `view` gives a tensor's tcab_tensor as
+    bytes or raises."""
+    try:
+        from . import _calls
+    except ImportError as e:
+        raise ImportError(f"{os.path.join(os.path.dirname(LIB_PATH), '_calls.so')} is missing or does not fit this torch: build it with "
+                          f"`python -m tcacomp_b200.build` (there is no fallback implementation): {e}") from e
+    lib = load()
+    names = ("layernorm_rows_stats", "layernorm_rows_backward", "layernorm_rows_backward_workspace", "gemm_bias_act_residual",
+             "gemm_bias_act_backward", "gemm_bias_act_backward_workspace", "gated_gemm", "gated_gemm_backward",
+             "gated_gemm_backward_workspace")
+    _calls.bind(view, check, *[C.cast(getattr(lib, "tcab_" + n), C.c_void_p).value for n in names])
+    return _calls
 
 
 def check(status: int) -> None:

@@ -28,6 +28,8 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-I", OBJ,
 ]
+CALLS_SRC = os.path.join(CSRC, "torch", "calls.cpp")
+CALLS = os.path.join(HERE, "_calls.so")  # Python extension module: host path of the operators of many tensors
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden"]
 
 
@@ -104,7 +106,33 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
         if r.returncode != 0:
             raise RuntimeError(f"linking libtcab.so failed:\n{r.stderr[-4000:]}")
     build_host(force or changed)
+    build_calls(force)
     return LIB
+
+
+def build_calls(force: bool = False) -> str:
+    """g++ build of csrc/torch/calls.cpp against this interpreter's torch. Rebuilt when the source, the C ABI or torch change."""
+    import sysconfig
+
+    import torch
+    troot = os.path.dirname(torch.__file__)
+    stamp = os.path.join(OBJ, "calls.sha")
+    dig = _digest(CALLS_SRC, [os.path.join(HERE, "..", "include", "tcab.h")]) + " " + torch.__version__ + " " + sys.version.split()[0]
+    if not force and os.path.exists(CALLS) and os.path.exists(stamp) and open(stamp).read() == dig:
+        return CALLS
+    nvcc = _nvcc()
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-o", CALLS, CALLS_SRC]
+    for d in (os.path.join(troot, "include"), os.path.join(troot, "include", "torch", "csrc", "api", "include"),
+              sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include")):
+        cmd += ["-isystem", d]
+    cmd += ["-L" + os.path.join(troot, "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"building _calls.so failed:\n{r.stderr[-4000:]}")
+    with open(stamp, "w") as f:
+        f.write(dig)
+    return CALLS
 
 
 def build_host(force: bool = False) -> str:

@@ -8,7 +8,6 @@ asynchronous on the given (or current) torch stream.
 from __future__ import annotations
 
 import ctypes as C
-import struct
 from typing import Optional, Sequence
 
 import torch
@@ -416,49 +415,24 @@ def _act_code(act: str, allowed: Sequence[str]) -> int:
     return _ACTS[act]
 
 
-# A tcab_tensor as bytes: what ctypes hands over as a pointer without building a structure field by field (the operators
-# below take five to eleven tensors; building ctypes structures was half of a small call's host time, 24 us of a
-# layernorm_rows_stats call against 12 with packed views).
-_PACK = {1: struct.Struct("<QiII12x").pack, 2: struct.Struct("<QiIII8x").pack, 3: struct.Struct("<QiIIII4x").pack,
-         4: struct.Struct("<QiIIIII").pack}
-
-
-def _packed(t: torch.Tensor, name: str, dev: int) -> bytes:
-    """_view as bytes, for a tensor that has to live on device `dev` (the first operand's)."""
-    if isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous():
-        code, shape = _DTYPES.get(t.dtype), t.shape
-        if code is not None and 0 < t.numel() < _TWO32 and len(shape) in _PACK:
-            if t.get_device() != dev:
-                raise ValueError(f"{name} is on {t.device} but the first operand is on cuda:{dev}")
-            return _PACK[len(shape)](t.data_ptr(), code, len(shape), *shape)
-    v = _view(t, name)  # refuses what is not a tensor this library takes; empty tensors come through
+def _bytes_view(t: torch.Tensor, name: str, dev: int) -> bytes:
+    """_view as bytes, for a tensor that has to live on device `dev` (the first operand's): what the native host path asks
+    for where a tensor is not of the usual kind. Refuses what this library does not take; empty tensors come through."""
+    v = _view(t, name)
     if t.get_device() != dev:
         raise ValueError(f"{name} is on {t.device} but the first operand is on cuda:{dev}")
     return bytes(v)
 
 
-# New contiguous tensors on the current device: the allocation entry torch's own generated code calls, a third of
-# torch.empty's argument handling (0.9 against 2.3 us); torch.empty where this torch does not have it.
-_empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+_CALLS = None
 
 
-def _new(shape: tuple, dtype: torch.dtype) -> torch.Tensor:
-    rank = len(shape)
-    if _empty_strided is None or rank > 2:
-        return torch.empty(shape, device="cuda", dtype=dtype)
-    return _empty_strided(shape, (1,) if rank == 1 else (shape[1], 1), dtype)
-
-
-def _packed_new(t: torch.Tensor, name: str, dev: int) -> bytes:
-    """_packed for a tensor made here: nothing to check but its size."""
-    shape = t.shape
-    if 0 < t.numel() < _TWO32:
-        return _PACK[len(shape)](t.data_ptr(), _DTYPES[t.dtype], len(shape), *shape)
-    return bytes(_view(t, name))
-
-
-def _packed_opt(t: Optional[torch.Tensor], name: str, dev: int) -> Optional[bytes]:
-    return None if t is None else _packed(t, name, dev)
+def _calls():
+    """The native host path (csrc/torch/calls.cpp), bound to the loaded library."""
+    global _CALLS
+    if _CALLS is None:
+        _CALLS = _lib.load_calls(_bytes_view)
+    return _CALLS
 
 
 def _device_of(t: torch.Tensor, name: str) -> int:
@@ -475,8 +449,11 @@ class _At:
 
     __slots__ = ("managers",)
 
-    def __init__(self, dev: int, stream: Optional[torch.cuda.Stream]):
-        self.managers = [torch.cuda.device(dev)] + ([] if stream is None else [torch.cuda.stream(stream)])
+    def __init__(self, stream: torch.cuda.Stream, t: torch.Tensor, name: str):
+        dev = _device_of(t, name)
+        if stream.device_index != dev:
+            raise ValueError(f"the stream is on cuda:{stream.device_index} but the first operand is on cuda:{dev}")
+        self.managers = [torch.cuda.device(dev), torch.cuda.stream(stream)]
 
     def __enter__(self):
         for m in self.managers:
@@ -488,45 +465,15 @@ class _At:
         return False
 
 
-def _at(dev: int, stream: Optional[torch.cuda.Stream]):
-    if stream is not None and stream.device_index != dev:
-        raise ValueError(f"the stream is on cuda:{stream.device_index} but the first operand is on cuda:{dev}")
-    if stream is None and dev == torch._C._cuda_getDevice():
-        return _ALREADY_CURRENT
-    return _At(dev, stream)
-
-
-def _raw_stream(stream: Optional[torch.cuda.Stream], dev: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
-
-
-def _matrices(a: torch.Tensor, an: str, b: torch.Tensor, bn: str) -> None:
-    for t, name in ((a, an), (b, bn)):
-        if not isinstance(t, torch.Tensor) or t.dim() != 2:
-            raise ValueError(f"{name} must be a rank-2 tensor")
-
-
 def layernorm_rows_stats(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps: float = 1e-5,
                          out: Optional[torch.Tensor] = None, mean: Optional[torch.Tensor] = None,
                          rstd: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> tuple:
     """layernorm_rows that also returns what its backward pass needs: (y, mean, rstd), the statistics fp32 with the
     extents of x without the innermost one (rank-1 x: [1])."""
-    dev = _device_of(x, "x")
-    fn = _lib.packed("tcab_layernorm_rows_stats")
-    with _at(dev, stream):
-        xv = _packed(x, "x", dev)
-        yp = mp = rp = _packed
-        if out is None:
-            out, yp = _new(tuple(x.shape), x.dtype), _packed_new
-        if mean is None:
-            mean, mp = _new(tuple(x.shape[:-1]) or (1,), torch.float32), _packed_new
-        if rstd is None:
-            rstd, rp = _new(tuple(x.shape[:-1]) or (1,), torch.float32), _packed_new
-        rc = fn(xv, _packed(gamma, "gamma", dev), _packed(beta, "beta", dev), eps, yp(out, "out", dev), mp(mean, "mean", dev),
-                rp(rstd, "rstd", dev), _raw_stream(stream, dev))
-    if rc:
-        _lib.check(rc)
-    return out, mean, rstd
+    if stream is not None:
+        with _At(stream, x, "x"):
+            return _calls().ln_stats(x, gamma, beta, eps, out, mean, rstd)
+    return (_CALLS or _calls()).ln_stats(x, gamma, beta, eps, out, mean, rstd)
 
 
 def layernorm_rows_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
@@ -534,25 +481,10 @@ def layernorm_rows_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tens
                             dbeta: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> tuple:
     """Backward pass of layernorm_rows_stats: (dx, dgamma, dbeta). dx has the type of x (it may be dy or x themselves),
     dgamma and dbeta are fp32."""
-    dev = _device_of(x, "x")
-    fn, need = _lib.packed("tcab_layernorm_rows_backward"), _lib.packed("tcab_layernorm_rows_backward_workspace")
-    with _at(dev, stream):
-        xv = _packed(x, "x", dev)
-        xp = gp = bp = _packed
-        if dx is None:
-            dx, xp = _new(tuple(x.shape), x.dtype), _packed_new
-        if dgamma is None:
-            dgamma, gp = _new((x.shape[-1],), torch.float32), _packed_new
-        if dbeta is None:
-            dbeta, bp = _new((x.shape[-1],), torch.float32), _packed_new
-        nbytes = need(xv)
-        ws = _new((nbytes,), torch.uint8) if nbytes else None
-        rc = fn(_packed(dy, "dy", dev), xv, _packed(gamma, "gamma", dev), _packed(mean, "mean", dev), _packed(rstd, "rstd", dev),
-                xp(dx, "dx", dev), gp(dgamma, "dgamma", dev), bp(dbeta, "dbeta", dev),
-                ws.data_ptr() if nbytes else None, nbytes, _raw_stream(stream, dev))
-    if rc:
-        _lib.check(rc)
-    return dx, dgamma, dbeta
+    if stream is not None:
+        with _At(stream, x, "x"):
+            return _calls().ln_backward(dy, x, gamma, mean, rstd, dx, dgamma, dbeta)
+    return (_CALLS or _calls()).ln_backward(dy, x, gamma, mean, rstd, dx, dgamma, dbeta)
 
 
 def gemm_bias_act_residual(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -562,29 +494,22 @@ def gemm_bias_act_residual(a: torch.Tensor, b: torch.Tensor, bias: Optional[torc
     none, relu, silu, gelu, gelu_tanh. preact [M,N] bf16, where given, receives a @ b + bias for the backward pass. c may
     be the residual itself (out=residual)."""
     code = _act_code(act, _PLAIN_ACTS)
-    dev = _device_of(a, "a")
-    _matrices(a, "a", b, "b")
-    fn = _lib.packed("tcab_gemm_bias_act_residual")
-    with _at(dev, stream):
-        op = _packed
-        if out is None:
-            out, op = _new((a.shape[0], b.shape[1]), torch.bfloat16), _packed_new
-        rc = fn(_packed(a, "a", dev), _packed(b, "b", dev), _packed_opt(bias, "bias", dev), _packed_opt(residual, "residual", dev),
-                code, _packed_opt(preact, "preact", dev), op(out, "out", dev), _raw_stream(stream, dev))
-    if rc:
-        _lib.check(rc)
-    return out
+    if stream is not None:
+        with _At(stream, a, "a"):
+            return _calls().gemm(a, b, bias, residual, code, out, preact)
+    return (_CALLS or _calls()).gemm(a, b, bias, residual, code, out, preact)
 
 
-def _wanted(want: Sequence[str], out: Optional[dict], shapes: dict) -> dict:
-    """The outputs a backward pass is to compute, by name: the caller's where given, new ones otherwise."""
-    res = dict(out) if out else {}
-    for name in (*res, *want):
-        if name not in shapes:
-            raise ValueError(f"unknown output {name!r} (one of {', '.join(shapes)})")
-        if name not in res:
-            res[name] = _new(shapes[name], torch.float32 if name.startswith("dbias") else torch.bfloat16)
-    return res
+def _asked(want: Sequence[str], out: Optional[dict], names: Sequence[str]) -> dict:
+    """The outputs of a backward pass by name: the caller's tensor, True for a new one, None where it is not wanted."""
+    asked = dict.fromkeys(names)
+    for name in want:
+        asked[name] = True
+    if out:
+        asked.update(out)
+    if len(asked) != len(names):
+        raise ValueError(f"unknown output {next(n for n in asked if n not in names)!r} (one of {', '.join(names)})")
+    return asked
 
 
 def gemm_bias_act_backward(dc: torch.Tensor, a: torch.Tensor, b: torch.Tensor, preact: Optional[torch.Tensor] = None,
@@ -593,21 +518,13 @@ def gemm_bias_act_backward(dc: torch.Tensor, a: torch.Tensor, b: torch.Tensor, p
     """Backward pass of gemm_bias_act_residual; returns {"da" [M,K] bf16, "db" [K,N] bf16, "dbias" [N] fp32} as requested
     (the gradient of the residual is dc). preact is what the forward pass stored; it is not needed for act="none"."""
     code = _act_code(act, _PLAIN_ACTS)
-    dev = _device_of(a, "a")
-    _matrices(a, "a", b, "b")
-    m, k, n = a.shape[0], a.shape[1], b.shape[1]
-    fn, need = _lib.packed("tcab_gemm_bias_act_backward"), _lib.packed("tcab_gemm_bias_act_backward_workspace")
-    with _at(dev, stream):
-        av, bv = _packed(a, "a", dev), _packed(b, "b", dev)
-        res = _wanted(want, out, {"da": (m, k), "db": (k, n), "dbias": (n,)})
-        nbytes = need(m, n, code, "dbias" in res)
-        ws = _new((nbytes,), torch.uint8) if nbytes else None
-        rc = fn(_packed(dc, "dc", dev), av, bv, _packed_opt(preact, "preact", dev), code, _packed_opt(res.get("da"), "da", dev),
-                _packed_opt(res.get("db"), "db", dev), _packed_opt(res.get("dbias"), "dbias", dev),
-                ws.data_ptr() if nbytes else None, nbytes, _raw_stream(stream, dev))
-    if rc:
-        _lib.check(rc)
-    return res
+    asked = _asked(want, out, ("da", "db", "dbias"))
+    if stream is not None:
+        with _At(stream, a, "a"):
+            res = _calls().gemm_backward(dc, a, b, preact, code, *asked.values())
+    else:
+        res = (_CALLS or _calls()).gemm_backward(dc, a, b, preact, code, *asked.values())
+    return {name: t for name, t in zip(asked, res) if t is not None}
 
 
 def gated_gemm(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, bias_gate: Optional[torch.Tensor] = None,
@@ -618,19 +535,10 @@ def gated_gemm(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, bias_g
     the biases [N] fp32 (both or neither); act one of silu, gelu, gelu_tanh, sigmoid, relu. gate and up [M,N] bf16 (both or
     neither) receive the two projections for the backward pass."""
     code = _act_code(act, _GATE_ACTS)
-    dev = _device_of(x, "x")
-    _matrices(x, "x", w_gate, "w_gate")
-    fn = _lib.packed("tcab_gated_gemm")
-    with _at(dev, stream):
-        op = _packed
-        if out is None:
-            out, op = _new((x.shape[0], w_gate.shape[1]), torch.bfloat16), _packed_new
-        rc = fn(_packed(x, "x", dev), _packed(w_gate, "w_gate", dev), _packed(w_up, "w_up", dev),
-                _packed_opt(bias_gate, "bias_gate", dev), _packed_opt(bias_up, "bias_up", dev), code, _packed_opt(gate, "gate", dev),
-                _packed_opt(up, "up", dev), op(out, "out", dev), _raw_stream(stream, dev))
-    if rc:
-        _lib.check(rc)
-    return out
+    if stream is not None:
+        with _At(stream, x, "x"):
+            return _calls().gated(x, w_gate, w_up, bias_gate, bias_up, code, out, gate, up)
+    return (_CALLS or _calls()).gated(x, w_gate, w_up, bias_gate, bias_up, code, out, gate, up)
 
 
 def gated_gemm_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, gate: torch.Tensor,
@@ -639,18 +547,10 @@ def gated_gemm_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor,
     """Backward pass of gated_gemm from the projections it stored; returns {"dx" [M,K], "dw_gate" and "dw_up" [K,N] bf16,
     "dbias_gate" and "dbias_up" [N] fp32} as requested (the weights' gradients both or neither, the biases' likewise)."""
     code = _act_code(act, _GATE_ACTS)
-    dev = _device_of(x, "x")
-    _matrices(x, "x", w_gate, "w_gate")
-    m, k, n = x.shape[0], x.shape[1], w_gate.shape[1]
-    fn, need = _lib.packed("tcab_gated_gemm_backward"), _lib.packed("tcab_gated_gemm_backward_workspace")
-    with _at(dev, stream):
-        xv, gv = _packed(x, "x", dev), _packed(w_gate, "w_gate", dev)
-        res = _wanted(want, out, {"dx": (m, k), "dw_gate": (k, n), "dw_up": (k, n), "dbias_gate": (n,), "dbias_up": (n,)})
-        nbytes = need(m, n, "dbias_gate" in res or "dbias_up" in res)
-        ws = _new((nbytes,), torch.uint8) if nbytes else None
-        rc = fn(_packed(dh, "dh", dev), xv, gv, _packed(w_up, "w_up", dev), _packed(gate, "gate", dev), _packed(up, "up", dev), code,
-                *[_packed_opt(res.get(name), name, dev) for name in ("dx", "dw_gate", "dw_up", "dbias_gate", "dbias_up")],
-                ws.data_ptr() if nbytes else None, nbytes, _raw_stream(stream, dev))
-    if rc:
-        _lib.check(rc)
-    return res
+    asked = _asked(want, out, ("dx", "dw_gate", "dw_up", "dbias_gate", "dbias_up"))
+    if stream is not None:
+        with _At(stream, x, "x"):
+            res = _calls().gated_backward(dh, x, w_gate, w_up, gate, up, code, *asked.values())
+    else:
+        res = (_CALLS or _calls()).gated_backward(dh, x, w_gate, w_up, gate, up, code, *asked.values())
+    return {name: t for name, t in zip(asked, res) if t is not None}

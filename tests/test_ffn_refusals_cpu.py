@@ -214,3 +214,17 @@ def test_extents_of_31_bits(tcab_lib):
     assert call(L, "tcab_gated_gemm", [a, b, b, None, None, 2, None, None, c, None]) == _lib.ERR_TOO_LARGE
     x, y, g, st = T_((1, n), 1, far), T_((1, n), 1, 2 * far), T_((n,), 1, 3 * far), T_((1,), 0, 4 * far)
     assert call(L, "tcab_layernorm_rows_stats", [x, g, T_((n,), 1, 5 * far), 1e-5, y, st, T_((1,), 0, 6 * far), None]) == _lib.ERR_TOO_LARGE
+
+
+def test_outputs_asked_for_by_name(tcab_lib):
+    import tcacomp_b200 as T
+    x = torch.zeros(8, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="unknown output 'dx'"):
+        T.gemm_bias_act_backward(x, x, x, x, "silu", want=("da", "dx"))
+    with pytest.raises(ValueError, match="unknown output 'da'"):
+        T.gated_gemm_backward(x, x, x, x, x, x, "silu", out={"da": x})
+    for stream in (None, torch.cuda.ExternalStream(0) if torch.cuda.is_available() else None):
+        with pytest.raises(ValueError, match="CUDA"):
+            T.gated_gemm_backward(x, x, x, x, x, x, "silu", stream=stream)
+    with pytest.raises(TypeError, match="x must be a torch.Tensor"):
+        T.layernorm_rows_stats(None, x, x)
