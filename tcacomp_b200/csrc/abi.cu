@@ -995,6 +995,7 @@ int tcab_gemm_bias_act_backward(const tcab_tensor* dc, const tcab_tensor* a, con
     TCAB_TRY(launch_act_backward(op, TCAB_ACT_NONE, dz, nullptr, nullptr, f32_of(dbias), m, n, ws, s));
     beside = n > 0;
   }
+  FfnTaken taken;
   if (da != nullptr) {
     FfnProblem p;
     p.a[0] = dz;
@@ -1004,7 +1005,7 @@ int tcab_gemm_bias_act_backward(const tcab_tensor* dc, const tcab_tensor* a, con
     p.N = k;
     p.K = n;
     p.beside = beside;
-    TCAB_TRY(launch_ffn_gemm(op, kFfnDx, p, s));
+    TCAB_TRY(launch_ffn_gemm(op, kFfnDx, p, s, &taken));
     beside = beside || (m > 0 && k > 0);
   }
   if (db != nullptr) {
@@ -1016,6 +1017,8 @@ int tcab_gemm_bias_act_backward(const tcab_tensor* dc, const tcab_tensor* a, con
     p.N = n;
     p.K = m;
     p.beside = beside;
+    p.taken = taken.sms;
+    p.taken_us = taken.us;
     TCAB_TRY(launch_ffn_gemm(op, kFfnDw, p, s));
   }
   return TCAB_OK;
@@ -1096,6 +1099,7 @@ int tcab_gated_gemm_backward(const tcab_tensor* dh, const tcab_tensor* x, const 
   TCAB_TRY(launch_gated_backward(op, act, bf16_of(dh), bf16_of(gate), bf16_of(up), dgate, dup, f32_of(dbias_gate), f32_of(dbias_up),
                                  m, n, ws + 2 * plane, s));
   bool beside = dbias_gate != nullptr && n > 0;  // the last launch of this call so far, if there is one, writes neither
+  FfnTaken taken;
   if (dx != nullptr) {
     FfnProblem p;
     p.a[0] = dgate;
@@ -1107,7 +1111,7 @@ int tcab_gated_gemm_backward(const tcab_tensor* dh, const tcab_tensor* x, const 
     p.N = k;
     p.K = n;
     p.beside = beside;
-    TCAB_TRY(launch_ffn_gemm(op, kFfnDx, p, s));
+    TCAB_TRY(launch_ffn_gemm(op, kFfnDx, p, s, &taken));
     beside = beside || (m > 0 && k > 0);
   }
   if (dw_gate != nullptr) {
@@ -1121,6 +1125,8 @@ int tcab_gated_gemm_backward(const tcab_tensor* dh, const tcab_tensor* x, const 
     p.N = n;
     p.K = m;
     p.beside = beside;
+    p.taken = taken.sms;
+    p.taken_us = taken.us;
     TCAB_TRY(launch_ffn_gemm(op, kFfnDw, p, s));
   }
   return TCAB_OK;

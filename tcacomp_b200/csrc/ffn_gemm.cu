@@ -52,27 +52,35 @@ constexpr int kShapes = 3, kCtas[kShapes] = {2, 2, 1}, kRows[kShapes] = {512, 25
 // 128 x 128, against 42.5, 22.5, 26.5; 1003 x 1000 x 2728 11.2 for 256 x 256, against 17.3, 16.7, 24.9; 2048 x 4096 x 4096
 // 46.5 for 512 x 256, against 47.8, 77.4, 103; 256 x 4096 x 4096 16.1 for the small one, against 41.8, 22.3, 19.0.
 // Over many rounds the 512 x 256 tile wins (8192^3: 1,395 TFLOP/s against 1,305 for 256 x 256): it moves the fewest bytes.
-int choose(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sm) {
+struct Choice {
+  int shape;
+  double us;
+  uint32_t ctas;  // at once at most
+};
+Choice choose(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sm, bool shared_l2 = false) {
   static const double kFixed[kShapes] = {8.3, 5.8, 3.6}, kBlock[kShapes] = {0.49, 0.30, 0.25}, kEpilogue[kShapes] = {4.0, 2.2, 1.0};
   const uint64_t sms = static_cast<uint64_t>(sm);
   const uint64_t outs = form == kFfnDw ? pairs : 1, blocks = (static_cast<uint64_t>(k) + 63) / 64 * (form == kFfnDx ? pairs : 1);
+  const FfnSmallPlan small = ffn_small_plan(form, m, n, k, pairs, sm, 0);
   int best = kShapes;
-  double best_us = ffn_small_plan(form, m, n, k, pairs, sm, 0).us;
+  double best_us = small.us;
+  uint64_t best_ctas = small.tiles * small.ks;
   for (int s = 0; s < kShapes; ++s) {
     const uint64_t bm = kRows[s], tn = static_cast<uint64_t>(form == kFfnGated ? kBN[s] / 2 : kBN[s]);
     const uint64_t tiles = (m + bm - 1) / bm * ((n + tn - 1) / tn) * outs, at_once = sms / kCtas[s];
     if (at_once == 0) continue;
     const uint64_t rounds = (tiles + at_once - 1) / at_once;
     // a round's end is hidden where two accumulators alternate; the 512 x 256 tile pays part of it every time
-    double round = static_cast<double>(blocks) * kBlock[s] + (s == 0 ? 3.0 : 0.8);
+    double round = static_cast<double>(blocks) * (s == 2 && shared_l2 ? 0.40 : kBlock[s]) + (s == 0 ? 3.0 : 0.8);
     if (round < kEpilogue[s]) round = kEpilogue[s];  // few blocks: the time of storing a tile
     const double us = kFixed[s] + static_cast<double>(rounds) * round;
     if (us < best_us - 1e-9) {
       best_us = us;
       best = s;
+      best_ctas = (tiles < at_once ? tiles : at_once) * kCtas[s];
     }
   }
-  return best;
+  return {best, best_us, static_cast<uint32_t>(best_ctas < sms ? best_ctas : sms)};
 }
 
 }  // namespace
@@ -81,7 +89,7 @@ int choose(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sm)
 // K blocks of 64 that each of them takes (ffn_small.cuh: columns are 128, of a gated pair 64 each).
 void ffn_plan(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sms, uint32_t* rows, uint32_t* cols, uint32_t* ranges,
               uint32_t* blocks) {
-  const int shape = choose(form, m, n, k, pairs, sms);
+  const int shape = choose(form, m, n, k, pairs, sms).shape;
   if (shape == kShapes) {
     const FfnSmallPlan p = ffn_small_plan(form, m, n, k, pairs, sms, 0);
     *rows = static_cast<uint32_t>(p.tm);
@@ -114,23 +122,38 @@ int ffn_device_status(int* out) {
   return TCAB_OK;
 }
 
-int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t s) {
+int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t s, FfnTaken* taken) {
   if (p.M == 0 || p.N == 0) return TCAB_OK;
   const Tune& tn = tune(kFfn);
-  const int shape = tn.p1 > 0 && tn.p1 <= kShapes + 1 ? tn.p1 - 1 : choose(form, p.M, p.N, p.K, p.b[1] != nullptr ? 2 : 1, sm_count());
-  if (shape == kShapes) return launch_ffn_small(op, form, p, s);
+  const uint32_t pairs = p.b[1] != nullptr ? 2 : 1;
+  int sms = sm_count();
+  Choice choice = choose(form, p.M, p.N, p.K, pairs, sms);
+  if (p.beside && p.taken > 0 && p.taken < static_cast<uint32_t>(sms)) {
+    // After the launch beside it with all SMs (some 2 us of its start are hidden), or with it on those that it leaves.
+    // Backward passes, us: 800 x 768 x 2048 19.6 after, 15.7 with it; 200 x 1024 x 4096 17.0, 13.5; 515 x 1032 x 2056 20.8,
+    // 19.9 with 256 x 256 tiles and 21.9 with 128 x 128, whose operand tiles both kernels then draw from L2.
+    const int rest = sms - static_cast<int>(p.taken);
+    const Choice alone = choose(form, p.M, p.N, p.K, pairs, rest, true);
+    if ((alone.us > p.taken_us ? alone.us : p.taken_us) < p.taken_us + choice.us - 2.0) {
+      choice = alone;
+      sms = rest;
+    }
+  }
+  if (taken != nullptr) *taken = {choice.ctas, choice.us};
+  const int shape = tn.p1 > 0 && tn.p1 <= kShapes + 1 ? tn.p1 - 1 : choice.shape;
+  if (shape == kShapes) return launch_ffn_small(op, form, p, sms, s);
   const uint32_t ctas = kCtas[shape], bm = kRows[shape], bn = kBN[shape], tile_n = form == kFfnGated ? bn / 2 : bn;
   FfnArgs args = {};
   args.M = p.M;
   args.N = p.N;
   args.K = p.K;
-  args.pairs = p.b[1] != nullptr ? 2 : 1;
+  args.pairs = pairs;
   args.bias[0] = p.bias[0];
   args.bias[1] = p.bias[1];
   args.residual = p.residual;
   args.save = p.z[0] != nullptr ? 1 : 0;
   args.beside = p.beside ? 1 : 0;
-  const int nb = p.b[1] != nullptr ? 2 : 1;
+  const int nb = static_cast<int>(pairs);
   if (p.K > 0) {
     if (form == kFfnDw) {
       TCAB_TRY_RC(make_tensor_map(op, &args.a[0], p.a[0], p.K, p.M, 64, 64));
@@ -151,7 +174,7 @@ int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t 
   if (k.fn == nullptr) return fail(TCAB_ERR_UNSUPPORTED, "%s: no kernel for activation %d", op, p.act);
   TCAB_TRY_RC(reserve_smem(op, k.fn, k.smem));
   const uint64_t tiles = static_cast<uint64_t>((p.M + bm - 1) / bm) * ((p.N + tile_n - 1) / tile_n) * (form == kFfnDw ? nb : 1);
-  uint64_t groups = (tn.p0 > 0 ? static_cast<uint64_t>(tn.p0) : static_cast<uint64_t>(sm_count())) / ctas;
+  uint64_t groups = (tn.p0 > 0 ? static_cast<uint64_t>(tn.p0) : static_cast<uint64_t>(sms)) / ctas;
   if (groups > tiles) groups = tiles;
   if (groups < 1) groups = 1;
   cudaLaunchConfig_t cfg = {};

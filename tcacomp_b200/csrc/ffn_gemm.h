@@ -30,9 +30,18 @@ struct FfnProblem {
   // end, so that whoever waits for this kernel has waited for both. What the operands need was complete before: a kernel
   // lets its successor start only when it runs itself, and the first of a call runs on only after everything before it.
   bool beside = false;
+  // SMs that the launch beside it holds and for how long by its estimate: the kernel may be cut for the others.
+  uint32_t taken = 0;
+  double taken_us = 0;
 };
 
-int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t s);
+// What a launch took, for the one that may run beside it.
+struct FfnTaken {
+  uint32_t sms = 0;
+  double us = 0;
+};
+
+int launch_ffn_gemm(const char* op, int form, const FfnProblem& p, cudaStream_t s, FfnTaken* taken = nullptr);
 int ffn_device_status(int* out);
 
 // ffn_small.cuh: few rows or few output tiles
@@ -44,7 +53,7 @@ struct FfnSmallPlan {
   double us = 0;                          // the estimate that chose them
 };
 FfnSmallPlan ffn_small_plan(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sms, int forced_ks);
-int launch_ffn_small(const char* op, int form, const FfnProblem& p, cudaStream_t s);
+int launch_ffn_small(const char* op, int form, const FfnProblem& p, int sms, cudaStream_t s);
 int ffn_small_status(int* out);
 void ffn_plan(int form, uint32_t m, uint32_t n, uint32_t k, uint32_t pairs, int sms, uint32_t* rows, uint32_t* cols, uint32_t* ranges,
               uint32_t* blocks);

@@ -60,9 +60,9 @@ FfnSmallPlan ffn_small_plan(int form, uint32_t m, uint32_t n, uint32_t k, uint32
   return p;
 }
 
-int launch_ffn_small(const char* op, int form, const FfnProblem& p, cudaStream_t s) {
+int launch_ffn_small(const char* op, int form, const FfnProblem& p, int sms, cudaStream_t s) {
   const uint32_t pairs = p.b[1] != nullptr ? 2 : 1;
-  const FfnSmallPlan plan = ffn_small_plan(form, p.M, p.N, p.K, pairs, sm_count(), tune(kFfn).p3);
+  const FfnSmallPlan plan = ffn_small_plan(form, p.M, p.N, p.K, pairs, sms, tune(kFfn).p3);
   const FfnSmallKernel k = small_kernel(form, plan.tm);
   const uint32_t room = (plan.per_sm == 2 ? 112u : 225u) * 1024 - 1024 - k.receive_bytes;
   uint32_t stages = room / k.stage_bytes;
