@@ -6,8 +6,8 @@ Each .cu is compiled to an object in tcacomp_b200/_obj/ (in parallel), then
 linked into one shared library beside this file; csrc/torch/calls.cpp becomes
 the extension module _calls.so, compiled against the installed torch. nvcc
 cross-compiles without a GPU. The library links the static CUDA runtime and the
-driver API (libcuda is resolved at load time on a GPU box; on a box without a
-driver the library still loads and every compute entry point reports TCAB_ERR_CUDA).
+driver API (libcuda is resolved at load time; without a driver the library still
+loads and every compute entry point reports TCAB_ERR_CUDA).
 """
 from __future__ import annotations
 
